@@ -131,6 +131,16 @@ def library() -> ctypes.CDLL:
         for f in (lib.b200_mgemm_create, lib.b200_mgemm_buffers, lib.b200_mgemm_run, lib.b200_mgemm_sync,
                   lib.b200_mgemm_destroy):
             f.restype = ci
+    if hasattr(lib, "b200_gemm_mx"):
+        lib.b200_mx_data_bytes.argtypes = [ci, ci]
+        lib.b200_mx_data_bytes.restype = sz
+        lib.b200_mx_scale_bytes.argtypes = [ci, ci, ci]
+        lib.b200_mx_scale_bytes.restype = sz
+        lib.b200_mx_quantize.argtypes = [ci, ci, ci, ci, vp, ll, cf, vp, vp, vp, vp, vp]
+        lib.b200_mx_dequantize.argtypes = [ci, ci, ci, ci, vp, vp, cf, vp, ll, vp]
+        lib.b200_gemm_mx.argtypes = [ci, ci, ci, ci, ci, vp, vp, vp, vp, vp, cf, cf, vp]
+        for f in (lib.b200_mx_quantize, lib.b200_mx_dequantize, lib.b200_gemm_mx):
+            f.restype = ci
     lib.b200_gemm_tuning_load.argtypes = [ctypes.c_char_p]
     lib.b200_gemm_tuning_load.restype = ci
     lib.b200_gemm_tuning_add.argtypes = [ci, ci, ci, ci, cfgp]

@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -48,7 +49,7 @@ def _run(cmd, cwd=None) -> None:
 
 def kernel_sources():
     return sorted(list(CSRC.glob("*.cu")) + list(CSRC.glob("sm100/*.cuh")) +
-                  [REPO_DIR / "include" / "b200_gemm.h"])
+                  [CSRC / "internal.h", REPO_DIR / "include" / "b200_gemm.h"])
 
 
 def build_library(force: bool = False, verbose: bool = False) -> Path:
@@ -57,10 +58,19 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     srcs = kernel_sources()
     if not force and _newer(LIB_PATH, srcs):
         return LIB_PATH
-    cmd = [_nvcc(), *NVCC_COMMON, *NVCC_ARCH, "-o", str(LIB_PATH), str(CSRC / "launcher.cu")]
-    if verbose:
-        cmd += ["-Xptxas", "-v"]
-    _run(cmd)
+    units = sorted(CSRC.glob("*.cu"))
+    objects = [LIB_DIR / (u.stem + ".o") for u in units]
+    headers = [s for s in srcs if Path(s).suffix != ".cu"]
+    flags = [f for f in NVCC_COMMON if f != "-shared"] + (["-Xptxas", "-v"] if verbose else [])
+
+    def compile_unit(unit: Path, obj: Path) -> None:
+        if force or not _newer(obj, [unit, *headers]):
+            _run([_nvcc(), *flags, *NVCC_ARCH, "-c", "-o", str(obj), str(unit)])
+
+    with ThreadPoolExecutor(max_workers=len(units)) as pool:
+        for job in [pool.submit(compile_unit, u, o) for u, o in zip(units, objects)]:
+            job.result()
+    _run([_nvcc(), *NVCC_COMMON, *NVCC_ARCH, "-o", str(LIB_PATH), *map(str, objects)])
     return LIB_PATH
 
 

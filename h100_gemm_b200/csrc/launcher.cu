@@ -28,6 +28,7 @@
 #include <vector>
 
 #include "../../include/b200_gemm.h"
+#include "internal.h"
 #include "sm100/gemm_kernel.cuh"
 
 namespace {
@@ -216,11 +217,6 @@ const KernelEntry* find_kernel(int bn, int pair, int mt) {
 // ------------------------------------------------------------------------------------------
 // Per-device state
 // ------------------------------------------------------------------------------------------
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
 struct DeviceState {
   bool ready = false;
   int sm_count = 0;
@@ -1128,6 +1124,28 @@ int grow(void** p, size_t* cap, size_t need) {
 }
 
 }  // namespace
+
+namespace b200 {
+
+int device_info(DeviceInfo* out) {
+  std::lock_guard<std::mutex> lock(g_mutex);
+  DeviceState* st = nullptr;
+  const int rc = get_device_state(&st);
+  if (rc != B200_OK) return rc;
+  out->ordinal = static_cast<int>(st - g_devices);
+  out->sm_count = st->sm_count;
+  out->smem_optin = st->smem_optin;
+  out->status = st->status;
+  out->encode = g_encode;
+  return B200_OK;
+}
+
+int cuda_failed(int error) {
+  g_last_cuda_error = error;
+  return B200_ERR_CUDA;
+}
+
+}  // namespace b200
 
 // ==========================================================================================
 // C ABI

@@ -1,0 +1,269 @@
+// Host side of the microscaled 4-bit operators (include/b200_gemm.h): quantisation, its inverse, and the product.
+#include <cstring>
+
+#include "internal.h"
+#include "sm100/mx_gemm.cuh"
+#include "sm100/mx_quant.cuh"
+
+namespace {
+
+using namespace b200;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+bool format_known(int format) { return format == B200_MXFP4 || format == B200_NVFP4; }
+
+// Powers of two within fp32's comfortable range, so that dividing by one is exact.
+bool tensor_scale_ok(int format, float t) {
+  uint32_t bits;
+  std::memcpy(&bits, &t, sizeof bits);
+  const int exponent = static_cast<int>(bits >> 23) - 127;
+  if ((bits & 0x807FFFFFu) != 0 || exponent < -64 || exponent > 64) return false;
+  return format == B200_NVFP4 || t == 1.0f;
+}
+
+// A launch in stream order with the set-up overlapping the kernel before it (every kernel here
+// waits for that kernel to complete before it touches global memory).
+struct Launch {
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attr[2];
+  Launch(long long grid, int threads, size_t smem, cudaStream_t stream, int cluster = 1) {
+    config.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+    config.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+  }
+};
+
+template <int FMT, int F16, int ROW, int COL>
+int launch_quantize(const QuantArgs& args, bool vec, long long grid, cudaStream_t stream) {
+  Launch l(grid, kQuantThreads, 0, stream);
+  if (vec) {
+    B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, &quantize_kernel<FMT, F16, ROW, COL, 1>, args));
+  } else {
+    B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, &quantize_kernel<FMT, F16, ROW, COL, 0>, args));
+  }
+  return B200_OK;
+}
+
+template <int FMT, int F16>
+int launch_quantize(const QuantArgs& args, bool vec, long long grid, cudaStream_t stream) {
+  if (args.data[0] && args.data[1]) return launch_quantize<FMT, F16, 1, 1>(args, vec, grid, stream);
+  if (args.data[0]) return launch_quantize<FMT, F16, 1, 0>(args, vec, grid, stream);
+  return launch_quantize<FMT, F16, 0, 1>(args, vec, grid, stream);
+}
+
+template <int FMT, int F16>
+int launch_dequantize(const DequantArgs& args, bool vec, long long grid, cudaStream_t stream) {
+  Launch l(grid, kQuantThreads, 0, stream);
+  if (vec) {
+    B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, &dequantize_kernel<FMT, F16, 1>, args));
+  } else {
+    B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, &dequantize_kernel<FMT, F16, 0>, args));
+  }
+  return B200_OK;
+}
+
+// Rank-3 tile map {inner, rows, 1}.
+int tile_map(const DeviceInfo& dev, CUtensorMap* out, CUtensorMapDataType type, const void* base, uint64_t inner,
+             uint64_t rows, uint64_t pitch_bytes, uint32_t box_inner, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  cuuint64_t dims[3] = {inner, rows, 1};
+  cuuint64_t strides[2] = {pitch_bytes, pitch_bytes * rows};
+  cuuint32_t box[3] = {box_inner, box_rows, 1};
+  cuuint32_t steps[3] = {1, 1, 1};
+  const CUresult r = dev.encode(out, type, 3, const_cast<void*>(base), dims, strides, box, steps,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200_OK : cuda_failed(static_cast<int>(r));
+}
+
+int code_map(const DeviceInfo& dev, CUtensorMap* out, const void* codes, long long rows, long long cols, int box_rows) {
+  const uint64_t pitch = static_cast<uint64_t>(mx_pitch(cols));
+  return tile_map(dev, out, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, pitch, static_cast<uint64_t>(rows), pitch, 128,
+                  static_cast<uint32_t>(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// The scales as rows of 1 KB; one box is one 128 x 256 tile's scales.
+int scale_map(const DeviceInfo& dev, CUtensorMap* out, int format, const void* scales, long long rows, long long cols) {
+  const uint64_t kilobytes = static_cast<uint64_t>(mx_scale_bytes(format, rows, cols) / 1024);
+  return tile_map(dev, out, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, 256, kilobytes, 1024, 256,
+                  static_cast<uint32_t>(mx_tile_bytes(format) / 1024), CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+struct MxProduct {
+  int R, S, K;
+  const void *x, *sx, *w, *sw;
+};
+
+template <int FMT, int BN, int F16>
+int launch_gemm(const DeviceInfo& dev, const MxProduct& p, MxGemmArgs args, cudaStream_t stream) {
+  using T = MxGemmTraits<FMT, BN>;
+  args.tiles_r = static_cast<int>(mx_row_tiles(p.R));
+  args.k_tiles = static_cast<int>(mx_col_tiles(p.K));
+  const long long tiles = static_cast<long long>(args.tiles_r) * ((p.S + BN - 1) / BN);
+  // Two CTAs to an SM where their rings and accumulators fit: 113 KB of shared memory and half of
+  // tensor memory each.
+  const bool two = T::smem_bytes(kMxScaleBuffers) <= 113 * 1024 && T::kTmemCols <= 256;
+  const long long slots = static_cast<long long>(dev.sm_count) * (two ? 2 : 1);
+  int split = 1;
+  while (split < 8 && tiles * split * 2 <= slots && args.k_tiles >= split * 2 * 4) split *= 2;
+  const int budget = two ? 113 * 1024 : dev.smem_optin;
+  int stages = (budget - T::smem_bytes(0)) / T::kStageBytes;
+  if (stages > kMxMaxStages) stages = kMxMaxStages;
+  if (stages < kMxScaleBuffers) return B200_ERR_SMEM;
+  args.stages = stages;
+  CUtensorMap mx, mw, msx, msw;
+  int rc = code_map(dev, &mx, p.x, p.R, p.K, 128);
+  if (rc == B200_OK) rc = code_map(dev, &mw, p.w, p.S, p.K, BN);
+  if (rc == B200_OK) rc = scale_map(dev, &msx, FMT, p.sx, p.R, p.K);
+  if (rc == B200_OK) rc = scale_map(dev, &msw, FMT, p.sw, p.S, p.K);
+  if (rc != B200_OK) return rc;
+  const auto kernel = &mx_gemm_kernel<FMT, BN, F16>;
+  B200_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.smem_optin));
+  Launch l(tiles * split, T::kThreads, static_cast<size_t>(T::smem_bytes(stages)), stream, split);
+  B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, kernel, mx, mw, msx, msw, args, split));
+  return B200_OK;
+}
+
+template <int FMT, int F16>
+int launch_gemm(const DeviceInfo& dev, const MxProduct& p, const MxGemmArgs& args, int width, cudaStream_t stream) {
+  switch (width) {
+    case 16: return launch_gemm<FMT, 16, F16>(dev, p, args, stream);
+    case 32: return launch_gemm<FMT, 32, F16>(dev, p, args, stream);
+    case 64: return launch_gemm<FMT, 64, F16>(dev, p, args, stream);
+    case 128: return launch_gemm<FMT, 128, F16>(dev, p, args, stream);
+    default: return launch_gemm<FMT, 256, F16>(dev, p, args, stream);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t b200_mx_data_bytes(int rows, int cols) {
+  return rows > 0 && cols > 0 ? static_cast<size_t>(rows * mx_pitch(cols)) : 0;
+}
+
+size_t b200_mx_scale_bytes(int format, int rows, int cols) {
+  return format_known(format) && rows > 0 && cols > 0 ? static_cast<size_t>(mx_scale_bytes(format, rows, cols)) : 0;
+}
+
+int b200_mx_quantize(int format, int f16, int rows, int cols, const void* X, long long ldx, float tensor_scale,
+                     void* data, void* scales, void* data_t, void* scales_t, void* stream) {
+  if (!format_known(format) || rows <= 0 || cols <= 0 || X == nullptr || ldx < cols) return B200_ERR_INVALID_ARG;
+  if ((data == nullptr) != (scales == nullptr) || (data_t == nullptr) != (scales_t == nullptr)) return B200_ERR_INVALID_ARG;
+  if (data == nullptr && data_t == nullptr) return B200_ERR_INVALID_ARG;
+  if (!aligned16(data) || !aligned16(scales) || !aligned16(data_t) || !aligned16(scales_t)) return B200_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(X) & 1u) || !tensor_scale_ok(format, tensor_scale)) return B200_ERR_INVALID_ARG;
+  QuantArgs args;
+  args.x = static_cast<const uint16_t*>(X);
+  args.rows = rows;
+  args.cols = cols;
+  args.ldx = ldx;
+  args.inv_t = 1.0f / tensor_scale;
+  args.data[0] = static_cast<uint8_t*>(data);
+  args.data[1] = static_cast<uint8_t*>(data_t);
+  args.scales[0] = static_cast<uint8_t*>(scales);
+  args.scales[1] = static_cast<uint8_t*>(scales_t);
+  args.pitch[0] = mx_pitch(cols);
+  args.pitch[1] = mx_pitch(rows);
+  args.col_tiles[0] = mx_col_tiles(cols);
+  args.col_tiles[1] = mx_col_tiles(rows);
+  args.row_tiles[0] = mx_row_tiles(rows);
+  args.row_tiles[1] = mx_row_tiles(cols);
+  const long long tiles_x = data != nullptr ? 2 * args.col_tiles[0] : args.row_tiles[1];
+  const long long tiles_y = data_t != nullptr ? 2 * args.col_tiles[1] : args.row_tiles[0];
+  if (tiles_x * tiles_y > 0x7FFFFFFFll) return B200_ERR_INVALID_ARG;
+  args.tiles_x = static_cast<int>(tiles_x);
+  DeviceInfo dev;
+  const int rc = device_info(&dev);
+  if (rc != B200_OK) return rc;
+  const bool vec = aligned16(X) && ldx % 8 == 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const long long grid = tiles_x * tiles_y;
+  if (format == B200_MXFP4) {
+    return f16 ? launch_quantize<kMxfp4, 1>(args, vec, grid, s) : launch_quantize<kMxfp4, 0>(args, vec, grid, s);
+  }
+  return f16 ? launch_quantize<kNvfp4, 1>(args, vec, grid, s) : launch_quantize<kNvfp4, 0>(args, vec, grid, s);
+}
+
+int b200_mx_dequantize(int format, int f16, int rows, int cols, const void* data, const void* scales, float tensor_scale,
+                       void* X, long long ldx, void* stream) {
+  if (!format_known(format) || rows <= 0 || cols <= 0 || X == nullptr || ldx < cols) return B200_ERR_INVALID_ARG;
+  if (data == nullptr || scales == nullptr || !aligned16(data) || !aligned16(scales)) return B200_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(X) & 1u) != 0) return B200_ERR_INVALID_ARG;
+  DequantArgs args;
+  args.data = static_cast<const uint8_t*>(data);
+  args.scales = static_cast<const uint8_t*>(scales);
+  args.rows = rows;
+  args.cols = cols;
+  args.pitch = mx_pitch(cols);
+  args.col_tiles = mx_col_tiles(cols);
+  args.tensor_scale = tensor_scale;
+  args.x = static_cast<uint16_t*>(X);
+  args.ldx = ldx;
+  const long long tiles_x = (cols + kQuantTile - 1) / kQuantTile, tiles_y = mx_row_tiles(rows);
+  if (tiles_x * tiles_y > 0x7FFFFFFFll) return B200_ERR_INVALID_ARG;
+  args.tiles_x = static_cast<int>(tiles_x);
+  DeviceInfo dev;
+  const int rc = device_info(&dev);
+  if (rc != B200_OK) return rc;
+  const bool vec = aligned16(X) && ldx % 8 == 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const long long grid = tiles_x * tiles_y;
+  if (format == B200_MXFP4) {
+    return f16 ? launch_dequantize<kMxfp4, 1>(args, vec, grid, s) : launch_dequantize<kMxfp4, 0>(args, vec, grid, s);
+  }
+  return f16 ? launch_dequantize<kNvfp4, 1>(args, vec, grid, s) : launch_dequantize<kNvfp4, 0>(args, vec, grid, s);
+}
+
+int b200_gemm_mx(int format, int f16, int M, int N, int K, const void* A, const void* A_scales, const void* B,
+                 const void* B_scales, void* C, float alpha, float beta, void* stream) {
+  if (!format_known(format) || M <= 0 || N <= 0 || K <= 0) return B200_ERR_INVALID_ARG;
+  if (A == nullptr || A_scales == nullptr || B == nullptr || B_scales == nullptr || C == nullptr) return B200_ERR_INVALID_ARG;
+  if (!aligned16(A) || !aligned16(A_scales) || !aligned16(B) || !aligned16(B_scales)) return B200_ERR_INVALID_ARG;
+  if ((reinterpret_cast<uintptr_t>(C) & 1u) != 0) return B200_ERR_INVALID_ARG;
+  if (mx_scale_bytes(format, M, K) / 1024 > 0x7FFFFFFFll || mx_scale_bytes(format, N, K) / 1024 > 0x7FFFFFFFll) {
+    return B200_ERR_INVALID_ARG;
+  }
+  DeviceInfo dev;
+  const int rc = device_info(&dev);
+  if (rc != B200_OK) return rc;
+  // Up to 128 rows ride on the MMA's N, in the narrowest tile that holds them, and C is stored
+  // transposed; with more rows A takes the MMA's M.
+  const bool few = M <= 128;
+  MxProduct p;
+  MxGemmArgs args;
+  std::memset(&args, 0, sizeof args);
+  if (few) {
+    p = MxProduct{N, M, K, B, B_scales, A, A_scales};
+  } else {
+    p = MxProduct{M, N, K, A, A_scales, B, B_scales};
+  }
+  args.R = p.R;
+  args.S = p.S;
+  args.transposed = few ? 1 : 0;
+  args.vec = !few && aligned16(C) && N % 8 == 0 ? 1 : 0;
+  args.C = static_cast<uint16_t*>(C);
+  args.ldc = N;
+  args.alpha = alpha;
+  args.beta = beta;
+  args.scale = (alpha != 1.0f || beta != 0.0f) ? 1 : 0;
+  args.status = dev.status;
+  const int width = few ? (M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128) : (N <= 128 ? 128 : 256);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (format == B200_MXFP4) {
+    return f16 ? launch_gemm<kMxfp4, 1>(dev, p, args, width, s) : launch_gemm<kMxfp4, 0>(dev, p, args, width, s);
+  }
+  return f16 ? launch_gemm<kNvfp4, 1>(dev, p, args, width, s) : launch_gemm<kNvfp4, 0>(dev, p, args, width, s);
+}
+
+}  // extern "C"

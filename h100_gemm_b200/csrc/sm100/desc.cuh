@@ -30,6 +30,25 @@ B200_HD constexpr uint32_t make_instr_desc(uint32_t umma_m, uint32_t umma_n, InF
          ((umma_n >> 3) << 17) | ((umma_m >> 4) << 24);
 }
 
+// 32-bit instruction descriptor of tcgen05.mma.kind::mxf4 / kind::mxf4nvf4 (packed e2m1 operands):
+//   [4,6)   which pair of a scale column's four bytes B's scales start at (0 or 2; 0 for 16-element blocks)
+//   [7,10)  A format, [10,12) B format (1 = e2m1)
+//   [17,23) N >> 3
+//   [23]    scale type (0 = unsigned e4m3, 1 = exponent only)
+//   [27,29) M >> 7   (1 for one CTA, 2 for a CTA pair)
+//   [29,31) as [4,6) for A
+B200_HD constexpr uint32_t make_instr_desc_mxf4(uint32_t umma_m, uint32_t umma_n, bool exponent_scales,
+                                                uint32_t scale_id) {
+  return (scale_id << 4) | (1u << 7) | (1u << 10) | ((umma_n >> 3) << 17) | ((exponent_scales ? 1u : 0u) << 23) |
+         ((umma_m >> 7) << 27) | (scale_id << 29);
+}
+
+// 64-bit shared-memory matrix descriptor of one scale group for tcgen05.cp: 32 rows of 16 bytes, no swizzle,
+// 128 bytes between consecutive 8-row groups.
+B200_HD constexpr uint64_t make_smem_desc_scales(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128u >> 4) << 32) | (1ull << 46);
+}
+
 // 64-bit shared-memory matrix descriptor for a K-major operand tile stored as rows of 128 bytes
 // (64 16-bit elements) with the 128-byte swizzle a TMA tile load produces:
 //   [0,14)  start address >> 4

@@ -38,6 +38,7 @@
 #include "desc.cuh"
 #include "ptx.cuh"
 #include "scheduler.cuh"
+#include "status.cuh"
 
 namespace b200 {
 
@@ -48,17 +49,6 @@ static constexpr int kMaxStages = 24;
 static constexpr int kEpiChunkCols = 64;    // columns per TMA store (128 bytes of bf16)
 static constexpr int kEpiSlabBytes = 32 * kEpiChunkCols * 2;       // one warp, one buffer: 4 KB
 static constexpr int kBarrierBytes = 512;
-
-// Device status codes written to the status word when a bounded wait gives up.
-enum DeviceStatus : unsigned int {
-  kStatusOk = 0,
-  kStatusProducerTimeout = 1,   // producer waited for empty[s]
-  kStatusMmaFullTimeout = 2,    // MMA issuer waited for full[s]
-  kStatusMmaTmemTimeout = 3,    // MMA issuer waited for tmem_empty[a]
-  kStatusEpilogueTimeout = 4,   // epilogue waited for tmem_full[a]
-  kStatusStreamKTimeout = 5,    // stream-K finisher waited for another worker's partial tile
-  kStatusSelfTestTimeout = 9,   // the bounded-wait self-test (an mbarrier nothing arrives on)
-};
 
 // Per-CTA cycle counters written when GemmArgs::profile is set: where each role spent its time.
 // (The reference passes a debug buffer "DB" to runKernel for the same purpose but its kernel never

@@ -1,0 +1,295 @@
+// Quantisation to microscaled 4-bit floating point and back.
+//
+// Mathematics, for a block with the largest magnitude a:
+//   MXFP4   scale = 2^clamp(floor(log2 a) - 2, -127, 125), from the exponent bits of a
+//   NVFP4   scale = s * t, s = RN_e4m3(a / (6 t)) saturating at 448, t the matrix' power of two
+//   code    = RN_e2m1(x / scale), ties to even, saturating at 6; s = 0 gives zeros
+//   a block that holds a NaN or an infinity gets the NaN scale (and zero codes)
+// Everything is exact for 16-bit inputs. Division by 2^e is. For NVFP4, x / t has at most 11
+// significant bits and a border between two codes times s at most 7, so a quotient that is not on a border
+// differs from it by 2^-11 relative or more; x * RN(1 / s) is within 2^-23 of the quotient and,
+// rounded to 12 bits, on the border exactly when the quotient is.
+//
+// Bound by memory: 2 bytes read and 0.53 (MXFP4) or 0.56 (NVFP4) written per element and direction. A CTA
+// takes 128 x 128 elements: 256 bytes of every row (whole lines), eight 16-byte loads in flight per
+// thread, and complete 512-byte scale groups in either direction, so scales leave as whole lines and
+// the padding of the scale layout is written by the CTAs at the edges instead of a memset. The
+// transposed form turns the tile in shared memory (34 KB, so six CTAs per SM); both forms at once
+// read the matrix once.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "mx_format.cuh"
+#include "ptx.cuh"
+
+namespace b200 {
+
+static constexpr int kQuantTile = 128;
+static constexpr int kQuantThreads = 256;
+static constexpr int kQuantPitch = kQuantTile * 2 + 16;  // bytes between rows of the staged tile
+
+struct QuantArgs {
+  const uint16_t* x;
+  long long rows, cols, ldx;
+  float inv_t;              // 1 / tensor scale
+  uint8_t* data[2];         // [0] row form, [1] transposed form
+  uint8_t* scales[2];
+  long long pitch[2];
+  long long col_tiles[2];   // scale tiles along a row
+  long long row_tiles[2];
+  int tiles_x;              // CTAs along the columns of x
+};
+
+template <int F16>
+__device__ __forceinline__ float half_bits_to_float(uint32_t bits) {
+  if constexpr (F16) {
+    return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+  } else {
+    return __uint_as_float(bits << 16);
+  }
+}
+
+// The block's scale byte and what its elements are multiplied with; `amax` = largest magnitude as bits.
+// clip > 0 asks for the elements to be clipped to it first (the product would leave fp32's range).
+template <int FMT, int F16>
+__device__ __forceinline__ void block_scale(uint32_t amax, float inv_t, uint32_t* byte, float* mult, bool* bad,
+                                            bool* saturated) {
+  *bad = amax >= (F16 ? 0x7C00u : 0x7F80u);
+  *saturated = false;
+  const float a = half_bits_to_float<F16>(amax);
+  if constexpr (FMT == kMxfp4) {
+    const int e = static_cast<int>(__float_as_uint(a) >> 23) - 2;  // biased exponent of the scale
+    const uint32_t b = static_cast<uint32_t>(e > 0 ? e : 0);
+    *byte = *bad ? 255u : b;
+    *mult = __uint_as_float((254u - b) << 23);
+  } else {
+    const float scaled = a * inv_t;
+    const uint32_t b = e4m3_byte(__fdiv_rn(scaled, 6.0f));
+    *byte = *bad ? 127u : b;
+    *mult = b == 0u ? 0.0f : __frcp_rn(e4m3_value(b));
+    *saturated = scaled > 2688.0f;
+  }
+}
+
+// Eight elements (two to a word) -> eight codes.
+template <int FMT, int F16>
+__device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], float inv_t, float mult, bool bad, bool saturated) {
+  float v[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    v[j] = half_bits_to_float<F16>((j & 1) ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu);
+    if constexpr (FMT == kNvfp4) v[j] *= inv_t;
+  }
+  if constexpr (FMT == kNvfp4) {
+    if (saturated) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j], -2688.0f), 2688.0f);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float y = v[j] * mult;
+      const float c = y * 4097.0f;  // round to 12 significant bits
+      v[j] = __fsub_rn(c, __fsub_rn(c, y));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= mult;
+  }
+  const uint32_t codes = e2m1_pack8(v);
+  return bad ? 0u : codes;
+}
+
+// ROW / COL: which forms are written. VEC: rows of x start on 16 bytes.
+template <int FMT, int F16, int ROW, int COL, int VEC>
+__global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_constant__ QuantArgs args) {
+  constexpr int kGroups = kQuantTile / (4 * mx_block(FMT));  // scale groups of this tile: 1 or 2
+  __shared__ __align__(16) uint8_t tile[COL ? kQuantTile * kQuantPitch : 16];
+  __shared__ __align__(16) uint8_t scale_row[ROW ? kGroups * kMxGroupBytes : 16];
+  __shared__ __align__(16) uint8_t scale_col[COL ? kGroups * kMxGroupBytes : 16];
+  const int t = static_cast<int>(threadIdx.x);
+  const long long tx = blockIdx.x % args.tiles_x, ty = blockIdx.x / args.tiles_x;
+  const long long r0 = ty * kQuantTile, c0 = tx * kQuantTile;
+  const int piece = t & 15;  // 8 columns
+  const long long col = c0 + piece * 8;
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+
+  uint32_t w[8][4];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const long long row = r0 + p * 16 + (t >> 4);
+    w[p][0] = w[p][1] = w[p][2] = w[p][3] = 0u;
+    if (row < args.rows) {
+      const uint16_t* src = args.x + row * args.ldx + col;
+      if (VEC && col + 8 <= args.cols) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4*>(src));
+        w[p][0] = q.x;
+        w[p][1] = q.y;
+        w[p][2] = q.z;
+        w[p][3] = q.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (col + j < args.cols) w[p][j / 2] |= static_cast<uint32_t>(__ldg(src + j)) << (16 * (j & 1));
+        }
+      }
+    }
+  }
+
+  if constexpr (COL) {
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      *reinterpret_cast<uint4*>(tile + (p * 16 + (t >> 4)) * kQuantPitch + piece * 16) =
+          make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+    }
+  }
+  if constexpr (ROW) {
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const int r = p * 16 + (t >> 4);
+      uint32_t m = __vmaxu2(__vmaxu2(w[p][0] & 0x7FFF7FFFu, w[p][1] & 0x7FFF7FFFu),
+                            __vmaxu2(w[p][2] & 0x7FFF7FFFu, w[p][3] & 0x7FFF7FFFu));
+      m = max(m & 0xFFFFu, m >> 16);
+      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+      if constexpr (FMT == kMxfp4) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+      uint32_t byte;
+      float mult;
+      bool bad, sat;
+      block_scale<FMT, F16>(m, args.inv_t, &byte, &mult, &bad, &sat);
+      const uint32_t codes = quantise8<FMT, F16>(w[p], args.inv_t, mult, bad, sat);
+      const long long row = r0 + r;
+      if (row < args.rows && col / 2 + 4 <= args.pitch[0]) {
+        *reinterpret_cast<uint32_t*>(args.data[0] + row * args.pitch[0] + col / 2) = codes;
+      }
+      constexpr int kLanes = mx_block(FMT) / 8;  // lanes that share a block
+      if (piece % kLanes == 0) {
+        const int block = piece / kLanes;
+        scale_row[(block / 4) * kMxGroupBytes + (r % 32) * 16 + (r / 32) * 4 + block % 4] = static_cast<uint8_t>(byte);
+      }
+    }
+  }
+  __syncthreads();
+  if constexpr (ROW) {
+    // (with both forms the grid covers the padding of either; tiles outside this form's own are not written)
+    if (t < kGroups * kMxGroupBytes / 16 && ty < args.row_tiles[0] && tx < 2 * args.col_tiles[0]) {
+      uint8_t* dst = args.scales[0] + (ty * args.col_tiles[0] * 2 + tx) * (kGroups * kMxGroupBytes);
+      reinterpret_cast<uint4*>(dst)[t] = reinterpret_cast<const uint4*>(scale_row)[t];
+    }
+  }
+  if constexpr (COL) {
+    // Thread: columns 2 cp and 2 cp + 1, 32 consecutive rows of x (= elements of the transposed row).
+    const int cp = t & 63, rb = t >> 6;
+    uint32_t codes[2][4];
+    uint32_t v[32];
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      v[j] = *reinterpret_cast<const uint32_t*>(tile + (rb * 32 + j) * kQuantPitch + cp * 4);
+    }
+    constexpr int kBlk = mx_block(FMT);
+#pragma unroll
+    for (int b = 0; b < 32 / kBlk; ++b) {
+      uint32_t m = 0u;
+#pragma unroll
+      for (int j = 0; j < kBlk; ++j) m = __vmaxu2(m, v[b * kBlk + j] & 0x7FFF7FFFu);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t byte;
+        float mult;
+        bool bad, sat;
+        block_scale<FMT, F16>(h ? m >> 16 : m & 0xFFFFu, args.inv_t, &byte, &mult, &bad, &sat);
+#pragma unroll
+        for (int g = 0; g < kBlk / 8; ++g) {
+          const uint32_t* s = &v[b * kBlk + g * 8];
+          const uint32_t sel = h ? 0x7632u : 0x5410u;  // the upper or lower halves of two words
+          const uint32_t e[4] = {__byte_perm(s[0], s[1], sel), __byte_perm(s[2], s[3], sel),
+                                 __byte_perm(s[4], s[5], sel), __byte_perm(s[6], s[7], sel)};
+          codes[h][b * (kBlk / 8) + g] = quantise8<FMT, F16>(e, args.inv_t, mult, bad, sat);
+        }
+        const int r = cp * 2 + h, block = rb * (32 / kBlk) + b;
+        scale_col[(block / 4) * kMxGroupBytes + (r % 32) * 16 + (r / 32) * 4 + block % 4] = static_cast<uint8_t>(byte);
+      }
+    }
+    __syncthreads();  // the tile has been read: it now takes the codes, 64 bytes per transposed row
+    constexpr int kOutPitch = 80;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      *reinterpret_cast<uint4*>(tile + (cp * 2 + h) * kOutPitch + rb * 16) =
+          make_uint4(codes[h][0], codes[h][1], codes[h][2], codes[h][3]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = t; i < kQuantTile * 4; i += kQuantThreads) {
+      const long long row = c0 + i / 4, at = r0 / 2 + (i % 4) * 16;
+      if (row < args.cols && at + 16 <= args.pitch[1]) {
+        *reinterpret_cast<uint4*>(args.data[1] + row * args.pitch[1] + at) =
+            *reinterpret_cast<const uint4*>(tile + (i / 4) * kOutPitch + (i % 4) * 16);
+      }
+    }
+    if (t < kGroups * kMxGroupBytes / 16 && tx < args.row_tiles[1] && ty < 2 * args.col_tiles[1]) {
+      uint8_t* dst = args.scales[1] + (tx * args.col_tiles[1] * 2 + ty) * (kGroups * kMxGroupBytes);
+      reinterpret_cast<uint4*>(dst)[t] = reinterpret_cast<const uint4*>(scale_col)[t];
+    }
+  }
+}
+
+struct DequantArgs {
+  const uint8_t* data;
+  const uint8_t* scales;
+  long long rows, cols, pitch, col_tiles;
+  float tensor_scale;
+  uint16_t* x;
+  long long ldx;
+  int tiles_x;
+};
+
+// Codes and scales -> 16-bit values: code * scale * tensor scale in fp32, rounded once (exact in bf16
+// unless it leaves bf16's range: 2 bits of code times at most 4 of scale). Same 128 x 128 tiles.
+template <int FMT, int F16, int VEC>
+__global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_constant__ DequantArgs args) {
+  const int t = static_cast<int>(threadIdx.x);
+  const long long tx = blockIdx.x % args.tiles_x, ty = blockIdx.x / args.tiles_x;
+  const long long col = tx * kQuantTile + (t & 15) * 8;
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
+  if (col >= args.cols) return;
+  uint32_t codes[8], byte[8];
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const long long row = ty * kQuantTile + p * 16 + (t >> 4);
+    codes[p] = byte[p] = 0u;
+    if (row < args.rows) {
+      codes[p] = __ldg(reinterpret_cast<const uint32_t*>(args.data + row * args.pitch + col / 2));
+      byte[p] = __ldg(args.scales + mx_scale_offset(FMT, row, col / mx_block(FMT), args.col_tiles));
+    }
+  }
+#pragma unroll
+  for (int p = 0; p < 8; ++p) {
+    const long long row = ty * kQuantTile + p * 16 + (t >> 4);
+    if (row >= args.rows) continue;
+    const float scale = mx_scale_value<FMT>(byte[p]);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float lo = e2m1_value(codes[p] >> (8 * j)) * scale * args.tensor_scale;
+      const float hi = e2m1_value(codes[p] >> (8 * j + 4)) * scale * args.tensor_scale;
+      if constexpr (F16) {
+        asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(w[j]) : "f"(lo), "f"(hi));
+      } else {
+        asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(w[j]) : "f"(lo), "f"(hi));
+      }
+    }
+    uint16_t* dst = args.x + row * args.ldx + col;
+    if (VEC && col + 8 <= args.cols) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (col + j < args.cols) dst[j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+      }
+    }
+  }
+}
+
+}  // namespace b200

@@ -265,6 +265,48 @@ B200_DEVICE void umma_f16(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uin
   }
 }
 
+// Block-scaled form for packed 4-bit operands: every run of 32 (MXFP4: `BLOCK16` = 0) or 16 (NVFP4)
+// elements along K carries one 8-bit scale, read from tensor memory at `tmem_sfa` / `tmem_sfb`; one
+// instruction takes K = 64. fp32 accumulate.
+template <int CTA_GROUP, int BLOCK16>
+B200_DEVICE void umma_mxf4(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t tmem_sfa,
+                           uint32_t tmem_sfb, uint32_t accumulate) {
+#define B200_UMMA_MXF4(GROUP, KIND)                                                                  \
+  asm volatile(                                                                                      \
+      "{\n\t"                                                                                        \
+      ".reg .pred p;\n\t"                                                                            \
+      "setp.ne.b32 p, %4, 0;\n\t"                                                                    \
+      "tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], %1, %2, %3, [%5], [%6], p;\n\t"         \
+      "}" ::"r"(tmem_d),                                                                             \
+      "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate), "r"(tmem_sfa), "r"(tmem_sfb)            \
+      : "memory")
+  if constexpr (CTA_GROUP == 1) {
+    if constexpr (BLOCK16) {
+      B200_UMMA_MXF4("1", "mxf4nvf4.block_scale.scale_vec::4X");
+    } else {
+      B200_UMMA_MXF4("1", "mxf4.block_scale.scale_vec::2X");
+    }
+  } else {
+    if constexpr (BLOCK16) {
+      B200_UMMA_MXF4("2", "mxf4nvf4.block_scale.scale_vec::4X");
+    } else {
+      B200_UMMA_MXF4("2", "mxf4.block_scale.scale_vec::2X");
+    }
+  }
+#undef B200_UMMA_MXF4
+}
+
+// 512 bytes of shared memory (32 rows of 16 bytes) -> four 32-bit columns of tensor memory, repeated in each of
+// the four groups of 32 lanes: one group of block scales. Ordered before later MMAs of this thread.
+template <int CTA_GROUP>
+B200_DEVICE void tmem_copy_scales(uint32_t taddr, uint64_t desc) {
+  if constexpr (CTA_GROUP == 1) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  } else {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  }
+}
+
 // Make an mbarrier of THIS CTA track completion of all MMAs this thread issued so far.
 B200_DEVICE void umma_commit_1cta(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
@@ -325,6 +367,17 @@ B200_DEVICE void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c),
                "r"(d)
                : "memory");
+}
+
+B200_DEVICE void st_shared_f32(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+
+// One float of the shared memory of any CTA of the cluster (shared::cluster address).
+B200_DEVICE float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
 }
 
 B200_DEVICE uint4 ld_shared_v4(uint32_t addr) {

@@ -258,6 +258,49 @@ int b200_reference_gpu_gemm_bf16(int M, int N, int K, const void* A, const void*
 int b200_reference_gpu_gemm_f16(int M, int N, int K, const void* A, const void* B, void* C, float alpha,
                                 float beta, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Microscaled 4-bit floating point. No counterpart in the reference, whose operands are 16-bit.
+ *
+ * A matrix [rows, cols] is held as e2m1 codes (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives) with one
+ * 8-bit scale per block of consecutive elements of a row:
+ *   B200_MXFP4  blocks of 32, scale 2^(byte - 127), 255 = NaN
+ *   B200_NVFP4  blocks of 16, scale an unsigned e4m3 number (127 = NaN), times one power of two for the
+ *               whole matrix, the tensor scale, which the caller keeps
+ * data    two codes to a byte, element 2i in the lower half, rows of ceil(cols / 2) bytes rounded up to a
+ *         multiple of 16; what a row has beyond cols is zero.
+ * scales  tiles of 128 rows x 256 columns, tile after tile along a row of tiles. Inside a tile: groups
+ *         of 512 bytes, each the scales of 4 consecutive blocks of all 128 rows, with row r's
+ *         block b at byte (r % 32) * 16 + (r / 32) * 4 + b % 4. Rows and columns are padded to whole tiles;
+ *         the padding's bytes are zero (a padding byte that stands for NaN would spoil results).
+ * Both start on 16 bytes. The two sizes: */
+typedef enum b200_mx_format { B200_MXFP4 = 0, B200_NVFP4 = 1 } b200_mx_format;
+size_t b200_mx_data_bytes(int rows, int cols);
+size_t b200_mx_scale_bytes(int format, int rows, int cols);
+
+/* X [rows, cols], 16-bit (f16 = 0: bf16, 1: IEEE fp16), `ldx` elements between rows, any alignment of the
+ * type -> its 4-bit form (data, scales) and/or the 4-bit form of its transpose [cols, rows] (data_t,
+ * scales_t: blocks run down X's columns, as the products that contract over X's rows need them). A pair
+ * may be NULL; with both, X is read once. For a block with the largest magnitude a:
+ *   MXFP4: scale = 2^(floor(log2 a) - 2), exponent clamped to [-127, 125]; tensor_scale must be 1
+ *   NVFP4: scale = RN_e4m3(a / (6 tensor_scale)), at most 448; tensor_scale a power of two in [2^-64, 2^64]
+ *   codes = RN_e2m1(x / scale), ties to even, saturating at 6; a zero scale gives zeros.
+ * A block that holds a NaN or an infinity gets the NaN scale, so it reads back as NaN. Every border is decided
+ * exactly. Asynchronous on `stream`; no workspace, no allocation. */
+int b200_mx_quantize(int format, int f16, int rows, int cols, const void* X, long long ldx, float tensor_scale,
+                     void* data, void* scales, void* data_t, void* scales_t, void* stream);
+
+/* The values: X = code * scale * tensor_scale, rounded once to bf16 or fp16. */
+int b200_mx_dequantize(int format, int f16, int rows, int cols, const void* data, const void* scales,
+                       float tensor_scale, void* X, long long ldx, void* stream);
+
+/* C [M, N] (bf16, or fp16 with f16 = 1; row-major, contiguous) = (A * B^T) * alpha + beta for two matrices of one
+ * format, A [M, K] and B [N, K]: the tensor cores multiply the codes and apply the block scales, fp32
+ * accumulation, one rounding. The tensor scales of A and B belong into alpha; beta is added as a
+ * scalar as in b200_gemm_bf16. Asynchronous on `stream`; no workspace, no allocation, results do not
+ * depend on timing. */
+int b200_gemm_mx(int format, int f16, int M, int N, int K, const void* A, const void* A_scales, const void* B,
+                 const void* B_scales, void* C, float alpha, float beta, void* stream);
+
 /* Synchronises the current device and reports the device-side status word: out[0] = 0 when no
  * bounded wait has given up since the last call; otherwise out[0] = role code, out[1] = block,
  * out[2] = tile, out[3] = detail. Returns B200_OK or B200_ERR_DEVICE_TIMEOUT; the word is
