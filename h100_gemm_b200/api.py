@@ -141,6 +141,12 @@ def library() -> ctypes.CDLL:
         lib.b200_gemm_mx.argtypes = [ci, ci, ci, ci, ci, vp, vp, vp, vp, vp, cf, cf, vp]
         for f in (lib.b200_mx_quantize, lib.b200_mx_dequantize, lib.b200_gemm_mx):
             f.restype = ci
+    if hasattr(lib, "b200_moe_layer"):
+        lib.b200_moe_workspace_bytes.argtypes = [ci, ci, ci, ci, ci]
+        lib.b200_moe_workspace_bytes.restype = sz
+        lib.b200_moe_layer.argtypes = [ci, ci, ci, ci, ci, ci, vp, vp, vp, ci, vp, vp, cf, vp, vp, cf, ci, vp, vp, vp, vp,
+                                       sz, vp]
+        lib.b200_moe_layer.restype = ci
     lib.b200_gemm_tuning_load.argtypes = [ctypes.c_char_p]
     lib.b200_gemm_tuning_load.restype = ci
     lib.b200_gemm_tuning_add.argtypes = [ci, ci, ci, ci, cfgp]

@@ -1,0 +1,145 @@
+// Host side of the mixture-of-experts layer (include/b200_gemm.h).
+#include <cstring>
+
+#include "internal.h"
+#include "sm100/moe.cuh"
+
+namespace {
+
+using namespace b200;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+size_t round_up(size_t x) { return (x + 255) / 256 * 256; }
+
+// Workspace: [h][ids][weights]
+size_t h_bytes(int T, int k, int I) { return round_up(static_cast<size_t>(T) * k * I * 2); }
+size_t pair_bytes(int T, int k) { return round_up(static_cast<size_t>(T) * k * 4); }
+
+bool sizes_ok(int T, int E, int k, int H, int I) {
+  return T >= 1 && T <= kMoeMaxTokens && E >= 1 && E <= kMoeMaxExperts && k >= 1 && k <= kMoeMaxTopK && k <= E && H >= 8 &&
+         I >= 8 && H % 8 == 0 && I % 8 == 0 && H <= (1 << 20) && I <= (1 << 20);
+}
+
+struct Launch {
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attr[2];
+  Launch(int grid, int smem, cudaStream_t stream, int cluster) {
+    config.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+    config.blockDim = dim3(kMoeThreads, 1, 1);
+    config.dynamicSmemBytes = static_cast<size_t>(smem);
+    config.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+  }
+};
+
+template <int W, int F16, int NT>
+int launch_down(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) {
+  constexpr int MT = MoeUnit<W>::kTiles;
+  const int units = (args.H + 16 * MT - 1) / (16 * MT);
+  const int smem = kMoeWarps * MT * NT * 32 * 16 + route_table_bytes(args.E, args.T * args.k);
+  // Clusters share a unit until every SM has two CTAs, but no warp is left without a step.
+  const int most = args.T * args.k < args.E ? args.T * args.k : args.E;
+  const long long steps = static_cast<long long>(most) * ((args.I + kMoeStep - 1) / kMoeStep);
+  int split = 1;
+  while (split < 8 && units * split * 2 <= dev.sm_count * 2 && steps >= 2ll * split * kMoeWarps) split *= 2;
+  const auto kernel = &moe_down_kernel<W, F16, NT>;
+  B200_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.smem_optin));
+  Launch l(units * split, smem, stream, split);
+  B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, kernel, args, split));
+  return B200_OK;
+}
+
+template <int W, int F16>
+int launch_all(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) {
+  const int clusters = (args.T + kRouterTokens - 1) / kRouterTokens;
+  Launch route(clusters * kRouterCluster, 0, stream, kRouterCluster);
+  B200_TRY_CUDA(cudaLaunchKernelEx(&route.config, &moe_router_kernel<F16>, args));
+
+  constexpr int MT = MoeUnit<W>::kTiles;
+  const int most = args.T * args.k < args.E ? args.T * args.k : args.E;
+  const long long units = static_cast<long long>(most) * ((args.I + 8 * MT - 1) / (8 * MT));
+  const int grid = static_cast<int>(units < 2ll * dev.sm_count ? units : 2ll * dev.sm_count);
+  const int smem = 2 * kMoeWarps * 32 * 16 * MT * moe_token_tiles(args.T) + route_table_bytes(args.E, args.T * args.k);
+  const auto kernel = &moe_gate_up_kernel<W, F16>;
+  B200_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.smem_optin));
+  Launch up(grid, smem, stream, 1);
+  B200_TRY_CUDA(cudaLaunchKernelEx(&up.config, kernel, args));
+
+  switch (moe_token_tiles(args.T)) {
+    case 1: return launch_down<W, F16, 1>(dev, args, stream);
+    case 2: return launch_down<W, F16, 2>(dev, args, stream);
+    case 4: return launch_down<W, F16, 4>(dev, args, stream);
+    default: return launch_down<W, F16, 8>(dev, args, stream);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t b200_moe_workspace_bytes(int T, int E, int top_k, int H, int I) {
+  return sizes_ok(T, E, top_k, H, I) ? h_bytes(T, top_k, I) + 2 * pair_bytes(T, top_k) : 0;
+}
+
+int b200_moe_layer(int f16, int T, int E, int top_k, int H, int I, const void* X, const void* router, const float* bias,
+                   int weight_format, const void* W1, const void* W1_scales, float W1_tensor_scale, const void* W2,
+                   const void* W2_scales, float W2_tensor_scale, int renormalize, void* out, int* ids, float* weights,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  if (!sizes_ok(T, E, top_k, H, I)) return B200_ERR_INVALID_ARG;
+  const bool four_bit = weight_format != B200_MOE_16BIT;
+  if (weight_format != B200_MOE_16BIT && weight_format != B200_MXFP4 && weight_format != B200_NVFP4) return B200_ERR_INVALID_ARG;
+  if (four_bit && f16) return B200_ERR_INVALID_ARG;
+  if (X == nullptr || router == nullptr || W1 == nullptr || W2 == nullptr || out == nullptr) return B200_ERR_INVALID_ARG;
+  if (four_bit && (W1_scales == nullptr || W2_scales == nullptr)) return B200_ERR_INVALID_ARG;
+  if (!aligned16(X) || !aligned16(router) || !aligned16(W1) || !aligned16(W2) || !aligned16(W1_scales) ||
+      !aligned16(W2_scales) || (reinterpret_cast<uintptr_t>(out) & 1u) || (reinterpret_cast<uintptr_t>(bias) & 3u) ||
+      (reinterpret_cast<uintptr_t>(ids) & 3u) || (reinterpret_cast<uintptr_t>(weights) & 3u)) {
+    return B200_ERR_INVALID_ARG;
+  }
+  if (workspace == nullptr || workspace_bytes < b200_moe_workspace_bytes(T, E, top_k, H, I)) return B200_ERR_WORKSPACE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return B200_ERR_INVALID_ARG;
+  DeviceInfo dev;
+  const int rc = device_info(&dev);
+  if (rc != B200_OK) return rc;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  MoeArgs args;
+  std::memset(&args, 0, sizeof args);
+  args.T = T;
+  args.E = E;
+  args.k = top_k;
+  args.H = H;
+  args.I = I;
+  args.renormalize = renormalize ? 1 : 0;
+  args.x = static_cast<const uint16_t*>(X);
+  args.router = static_cast<const uint16_t*>(router);
+  args.bias = bias;
+  args.w1.data = static_cast<const uint8_t*>(W1);
+  args.w1.scales = static_cast<const uint8_t*>(W1_scales);
+  args.w1.pitch = four_bit ? mx_pitch(H) : 2ll * H;
+  args.w1.col_tiles = mx_col_tiles(H);
+  args.w2.data = static_cast<const uint8_t*>(W2);
+  args.w2.scales = static_cast<const uint8_t*>(W2_scales);
+  args.w2.pitch = four_bit ? mx_pitch(I) : 2ll * I;
+  args.w2.col_tiles = mx_col_tiles(I);
+  const float lift = weight_format == B200_NVFP4 ? MoeUnit<kMoeNvfp4>::kLift : 1.0f;
+  args.lift1 = four_bit ? lift * W1_tensor_scale : 1.0f;
+  args.lift2 = four_bit ? lift * W2_tensor_scale : 1.0f;
+  args.h = reinterpret_cast<uint16_t*>(ws);
+  args.ids = ids != nullptr ? ids : reinterpret_cast<int*>(ws + h_bytes(T, top_k, I));
+  args.weights = weights != nullptr ? weights : reinterpret_cast<float*>(ws + h_bytes(T, top_k, I) + pair_bytes(T, top_k));
+  args.out = static_cast<uint16_t*>(out);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (weight_format == B200_MXFP4) return launch_all<kMoeMxfp4, 0>(dev, args, s);
+  if (weight_format == B200_NVFP4) return launch_all<kMoeNvfp4, 0>(dev, args, s);
+  return f16 ? launch_all<kMoe16, 1>(dev, args, s) : launch_all<kMoe16, 0>(dev, args, s);
+}
+
+}  // extern "C"

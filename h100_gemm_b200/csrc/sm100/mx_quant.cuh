@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_co
     if (row < args.rows) {
       const uint16_t* src = args.x + row * args.ldx + col;
       if (VEC && col + 8 <= args.cols) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4*>(src));
+        const uint4 q = ptx::ld_stream_v4(src);
         w[p][0] = q.x;
         w[p][1] = q.y;
         w[p][2] = q.z;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_co
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          if (col + j < args.cols) w[p][j / 2] |= static_cast<uint32_t>(__ldg(src + j)) << (16 * (j & 1));
+          if (col + j < args.cols) w[p][j / 2] |= static_cast<uint32_t>(src[j]) << (16 * (j & 1));
         }
       }
     }
@@ -260,8 +260,8 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_
     const long long row = ty * kQuantTile + p * 16 + (t >> 4);
     codes[p] = byte[p] = 0u;
     if (row < args.rows) {
-      codes[p] = __ldg(reinterpret_cast<const uint32_t*>(args.data + row * args.pitch + col / 2));
-      byte[p] = __ldg(args.scales + mx_scale_offset(FMT, row, col / mx_block(FMT), args.col_tiles));
+      codes[p] = *reinterpret_cast<const uint32_t*>(args.data + row * args.pitch + col / 2);
+      byte[p] = args.scales[mx_scale_offset(FMT, row, col / mx_block(FMT), args.col_tiles)];
     }
   }
 #pragma unroll

@@ -380,6 +380,17 @@ B200_DEVICE float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
+// 16 bytes that are read once (not kept in L1). A coherent load: under programmatic dependent launch an earlier
+// launch of the same kernel may have left lines of a buffer in this SM's L1 that has been rewritten since,
+// and the read-only path does not promise to notice.
+B200_DEVICE uint4 ld_stream_v4(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
 B200_DEVICE uint4 ld_shared_v4(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"

@@ -1,0 +1,97 @@
+"""A mixture-of-experts layer for a few tokens, over the C ABI (b200_moe_layer)."""
+from __future__ import annotations
+
+from . import api
+from .api import STATUS_WORKSPACE, GemmError
+from .mx import FORMATS, MxTensor, _half_type, _invalid, _on, _require_cuda
+
+MAX_TOKENS, MAX_EXPERTS, MAX_TOP_K = 64, 512, 32
+
+
+def moe_workspace_bytes(tokens: int, experts: int, top_k: int, hidden: int, inner: int) -> int:
+    return int(api.library().b200_moe_workspace_bytes(tokens, experts, top_k, hidden, inner))
+
+
+def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: bool = True, out=None,
+              return_routing: bool = False, workspace=None, stream=None):
+    """out[T, H] = sum over each token's top_k experts e of p[t, e] * W2[e] (silu(G[e] x[t]) * (U[e] x[t])).
+
+    ``x`` [T, H] (at most 64 tokens), ``router`` [E, H], ``bias`` [E] fp32 added to the router's logits (-inf
+    takes an expert out), ``w_gate_up`` [E, 2 I, H] (the gate's I rows, then the up projection's),
+    ``w_down`` [E, H, I]: bfloat16 or float16, one type. Or, with bfloat16 tokens, 4-bit experts: ``w_gate_up`` an
+    MxTensor of E * 2 I rows and H columns, ``w_down`` one of E * H rows and I columns. ``renormalize``: the
+    softmax runs over the chosen experts, otherwise over all of them.
+
+    With ``return_routing`` the result is ``(out, ids, weights)``: the chosen experts [T, top_k] (int32, largest
+    logit first, -1 where fewer experts than top_k are left) and their weights (fp32). A token without any
+    expert gets zeros. Expert weights have to be finite. include/b200_gemm.h has the rounding and the limits.
+    """
+    import torch
+    f16 = _half_type(x.dtype, "x")
+    if x.dim() != 2 or router.dim() != 2 or router.shape[1] != x.shape[1]:
+        raise _invalid("x must be [tokens, hidden] and router [experts, hidden]")
+    T, H = x.shape
+    E = router.shape[0]
+    if not 1 <= T <= MAX_TOKENS:
+        raise _invalid(f"1 to {MAX_TOKENS} tokens, got {T}")
+    if not 1 <= E <= MAX_EXPERTS or not 1 <= top_k <= min(E, MAX_TOP_K):
+        raise _invalid(f"1 to {MAX_EXPERTS} experts and a top_k of 1 to {MAX_TOP_K}, at most all experts")
+    four_bit = isinstance(w_gate_up, MxTensor)
+    if four_bit != isinstance(w_down, MxTensor):
+        raise _invalid("w_gate_up and w_down must both be 4-bit or both not")
+    if four_bit:
+        if f16:
+            raise _invalid("4-bit experts take bfloat16 tokens")
+        if w_gate_up.format != w_down.format:
+            raise _invalid(f"w_gate_up is {w_gate_up.format}, w_down is {w_down.format}")
+        I = w_down.cols
+        if w_gate_up.cols != H or w_gate_up.rows != E * 2 * I or w_down.rows != E * H:
+            raise _invalid(f"w_gate_up must be a [{E} * 2 I, {H}] and w_down a [{E} * {H}, I] matrix")
+    else:
+        if w_gate_up.dim() != 3 or w_down.dim() != 3:
+            raise _invalid("w_gate_up must be [experts, 2 I, hidden] and w_down [experts, hidden, I]")
+        I = w_down.shape[2]
+        if tuple(w_gate_up.shape) != (E, 2 * I, H) or tuple(w_down.shape) != (E, H, I):
+            raise _invalid(f"w_gate_up must be [{E}, 2 I, {H}] and w_down [{E}, {H}, I]")
+    if H % 8 or I % 8 or H == 0 or I == 0:
+        raise _invalid("hidden and inner sizes must be multiples of 8")
+    _require_cuda(x, "x")
+    for name, t, dtype in (("x", x, x.dtype), ("router", router, x.dtype), ("bias", bias, torch.float32),
+                           ("w_gate_up", w_gate_up.data if four_bit else w_gate_up, torch.uint8 if four_bit else x.dtype),
+                           ("w_down", w_down.data if four_bit else w_down, torch.uint8 if four_bit else x.dtype)):
+        if t is None:
+            continue
+        _require_cuda(t, name, x.device)
+        if t.dtype != dtype or not t.is_contiguous():
+            raise _invalid(f"{name} must be a contiguous {dtype} tensor")
+        if name != "bias" and t.data_ptr() % 16:
+            raise _invalid(f"{name} must start on 16 bytes")
+    if bias is not None and tuple(bias.shape) != (E,):
+        raise _invalid(f"bias must have shape ({E},)")
+    need = moe_workspace_bytes(T, E, top_k, H, I)
+    with _on(x.device, stream) as s:
+        if out is None:
+            out = torch.empty((T, H), dtype=x.dtype, device=x.device)
+        _require_cuda(out, "out", x.device)
+        if out.dtype != x.dtype or tuple(out.shape) != (T, H) or not out.is_contiguous():
+            raise _invalid(f"out must be a contiguous [{T}, {H}] {x.dtype} tensor")
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        _require_cuda(workspace, "workspace", x.device)
+        nbytes = workspace.numel() * workspace.element_size()
+        if nbytes < need or not workspace.is_contiguous():
+            raise GemmError(STATUS_WORKSPACE, f"workspace needs {need} contiguous bytes")
+        ids = weights = None
+        if return_routing:
+            ids = torch.empty((T, top_k), dtype=torch.int32, device=x.device)
+            weights = torch.empty((T, top_k), dtype=torch.float32, device=x.device)
+        if four_bit:
+            w1 = (FORMATS[w_gate_up.format], w_gate_up.data.data_ptr(), w_gate_up.scales.data_ptr(), w_gate_up.tensor_scale)
+            w2 = (w_down.data.data_ptr(), w_down.scales.data_ptr(), w_down.tensor_scale)
+        else:
+            w1, w2 = (-1, w_gate_up.data_ptr(), None, 1.0), (w_down.data_ptr(), None, 1.0)
+        api._check(api.library().b200_moe_layer(
+            f16, T, E, top_k, H, I, x.data_ptr(), router.data_ptr(), bias.data_ptr() if bias is not None else None, *w1,
+            *w2, int(bool(renormalize)), out.data_ptr(), ids.data_ptr() if ids is not None else None,
+            weights.data_ptr() if weights is not None else None, workspace.data_ptr(), nbytes, s))
+    return (out, ids, weights) if return_routing else out

@@ -301,6 +301,27 @@ int b200_mx_dequantize(int format, int f16, int rows, int cols, const void* data
 int b200_gemm_mx(int format, int f16, int M, int N, int K, const void* A, const void* A_scales, const void* B,
                  const void* B_scales, void* C, float alpha, float beta, void* stream);
 
+/* A mixture-of-experts layer for a few tokens (a decode step), from the router to the weighted sum. No
+ * counterpart in the reference.
+ *   l[t, e] = X[t] . router[e] + bias[e]                  fp32; bias may be NULL, -inf takes an expert out
+ *   S[t]    = the top_k largest l[t, .], ties to the lower index, -inf never chosen, NaN before all others
+ *   p[t, e] = exp(l[t, e]) / sum of exp(l[t, .]) over S[t] (renormalize) or over all experts
+ *   h[t, e] = p[t, e] silu(W1[e, 0 : I] X[t]) (W1[e, I : 2 I] X[t])      rounded to 16 bits once
+ *   out[t]  = sum over S[t] of W2[e] h[t, e]              fp32 sum, rounded once; 0 when S[t] is empty
+ * X [T, H], router [E, H], W1 [E, 2 I, H] (gate rows, then up rows), W2 [E, H, I], out [T, H]: bf16, or fp16
+ * with f16 = 1, contiguous, X and weights on 16 bytes. weight_format B200_MXFP4 / B200_NVFP4: W1 and W2
+ * are 4-bit matrices of E * 2 I and E * H rows in the layout above, with their tensor scales (bf16 only).
+ * ids [T, top_k] (-1 = no expert) and weights [T, top_k] receive the routing, largest logit first; either may
+ * be NULL. Limits: T <= 64, E <= 512, top_k <= 32, H and I multiples of 8. Expert weights have to be
+ * finite (a token's zeros meet them). The workspace starts on 256 bytes and is free again when the work on `stream`
+ * is done; its contents do not matter. Asynchronous, no allocation, results do not depend on timing. */
+#define B200_MOE_16BIT (-1)
+size_t b200_moe_workspace_bytes(int T, int E, int top_k, int H, int I);
+int b200_moe_layer(int f16, int T, int E, int top_k, int H, int I, const void* X, const void* router, const float* bias,
+                   int weight_format, const void* W1, const void* W1_scales, float W1_tensor_scale, const void* W2,
+                   const void* W2_scales, float W2_tensor_scale, int renormalize, void* out, int* ids, float* weights,
+                   void* workspace, size_t workspace_bytes, void* stream);
+
 /* Synchronises the current device and reports the device-side status word: out[0] = 0 when no
  * bounded wait has given up since the last call; otherwise out[0] = role code, out[1] = block,
  * out[2] = tile, out[3] = detail. Returns B200_OK or B200_ERR_DEVICE_TIMEOUT; the word is
