@@ -4,6 +4,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
+
 #include "../../include/b200_gemm.h"
 
 namespace b200 {
@@ -34,5 +36,15 @@ int cuda_failed(int error);
       return ::b200::cuda_failed(static_cast<int>(e__));                       \
     }                                                                          \
   } while (0)
+
+// Lets a kernel use all of the device's shared memory; asked for once per device (`done`: the kernel's own flags).
+template <typename Kernel>
+int allow_shared_memory(const DeviceInfo& dev, Kernel kernel, std::atomic<bool> (&done)[64]) {
+  if (!done[dev.ordinal].load(std::memory_order_acquire)) {
+    B200_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.smem_optin));
+    done[dev.ordinal].store(true, std::memory_order_release);
+  }
+  return B200_OK;
+}
 
 }  // namespace b200

@@ -51,7 +51,9 @@ int launch_down(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream)
   int split = 1;
   while (split < 8 && units * split * 2 <= dev.sm_count * 2 && steps >= 2ll * split * kMoeWarps) split *= 2;
   const auto kernel = &moe_down_kernel<W, F16, NT>;
-  B200_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.smem_optin));
+  static std::atomic<bool> allowed[64];
+  const int rc = allow_shared_memory(dev, kernel, allowed);
+  if (rc != B200_OK) return rc;
   Launch l(units * split, smem, stream, split);
   B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, kernel, args, split));
   return B200_OK;
@@ -69,7 +71,9 @@ int launch_all(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) 
   const int grid = static_cast<int>(units < 2ll * dev.sm_count ? units : 2ll * dev.sm_count);
   const int smem = 2 * kMoeWarps * 32 * 16 * MT * moe_token_tiles(args.T) + route_table_bytes(args.E, args.T * args.k);
   const auto kernel = &moe_gate_up_kernel<W, F16>;
-  B200_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.smem_optin));
+  static std::atomic<bool> allowed[64];
+  const int rc = allow_shared_memory(dev, kernel, allowed);
+  if (rc != B200_OK) return rc;
   Launch up(grid, smem, stream, 1);
   B200_TRY_CUDA(cudaLaunchKernelEx(&up.config, kernel, args));
 

@@ -127,7 +127,9 @@ int launch_gemm(const DeviceInfo& dev, const MxProduct& p, MxGemmArgs args, cuda
   if (rc == B200_OK) rc = scale_map(dev, &msw, FMT, p.sw, p.S, p.K);
   if (rc != B200_OK) return rc;
   const auto kernel = &mx_gemm_kernel<FMT, BN, F16>;
-  B200_TRY_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, dev.smem_optin));
+  static std::atomic<bool> allowed[64];
+  rc = allow_shared_memory(dev, kernel, allowed);
+  if (rc != B200_OK) return rc;
   Launch l(tiles * split, T::kThreads, static_cast<size_t>(T::smem_bytes(stages)), stream, split);
   B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, kernel, mx, mw, msx, msw, args, split));
   return B200_OK;

@@ -3,7 +3,7 @@ from __future__ import annotations
 
 from . import api
 from .api import STATUS_WORKSPACE, GemmError
-from .mx import FORMATS, MxTensor, _half_type, _invalid, _on, _require_cuda
+from .mx import FORMATS, MxTensor, _half_type, _invalid, _output, _require_cuda, _run
 
 MAX_TOKENS, MAX_EXPERTS, MAX_TOP_K = 64, 512, 32
 
@@ -55,43 +55,46 @@ def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: 
             raise _invalid(f"w_gate_up must be [{E}, 2 I, {H}] and w_down [{E}, {H}, I]")
     if H % 8 or I % 8 or H == 0 or I == 0:
         raise _invalid("hidden and inner sizes must be multiples of 8")
-    _require_cuda(x, "x")
+    device = x.device
+    _require_cuda(device, "x")
     for name, t, dtype in (("x", x, x.dtype), ("router", router, x.dtype), ("bias", bias, torch.float32),
-                           ("w_gate_up", w_gate_up.data if four_bit else w_gate_up, torch.uint8 if four_bit else x.dtype),
-                           ("w_down", w_down.data if four_bit else w_down, torch.uint8 if four_bit else x.dtype)):
+                           ("w_gate_up", None if four_bit else w_gate_up, x.dtype),
+                           ("w_down", None if four_bit else w_down, x.dtype)):
         if t is None:
             continue
-        _require_cuda(t, name, x.device)
-        if t.dtype != dtype or not t.is_contiguous():
+        _require_cuda(t.device, name, device)
+        if t.dtype is not dtype or not t.is_contiguous():
             raise _invalid(f"{name} must be a contiguous {dtype} tensor")
-        if name != "bias" and t.data_ptr() % 16:
+        if t is not bias and t.data_ptr() % 16:
             raise _invalid(f"{name} must start on 16 bytes")
     if bias is not None and tuple(bias.shape) != (E,):
         raise _invalid(f"bias must have shape ({E},)")
+    if out is not None:
+        _output(out, (T, H), x.dtype, device, True)
     need = moe_workspace_bytes(T, E, top_k, H, I)
-    with _on(x.device, stream) as s:
-        if out is None:
-            out = torch.empty((T, H), dtype=x.dtype, device=x.device)
-        _require_cuda(out, "out", x.device)
-        if out.dtype != x.dtype or tuple(out.shape) != (T, H) or not out.is_contiguous():
-            raise _invalid(f"out must be a contiguous [{T}, {H}] {x.dtype} tensor")
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-        _require_cuda(workspace, "workspace", x.device)
-        nbytes = workspace.numel() * workspace.element_size()
-        if nbytes < need or not workspace.is_contiguous():
+    if workspace is not None:
+        _require_cuda(workspace.device, "workspace", device)
+        if workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
             raise GemmError(STATUS_WORKSPACE, f"workspace needs {need} contiguous bytes")
-        ids = weights = None
-        if return_routing:
-            ids = torch.empty((T, top_k), dtype=torch.int32, device=x.device)
-            weights = torch.empty((T, top_k), dtype=torch.float32, device=x.device)
-        if four_bit:
-            w1 = (FORMATS[w_gate_up.format], w_gate_up.data.data_ptr(), w_gate_up.scales.data_ptr(), w_gate_up.tensor_scale)
-            w2 = (w_down.data.data_ptr(), w_down.scales.data_ptr(), w_down.tensor_scale)
-        else:
-            w1, w2 = (-1, w_gate_up.data_ptr(), None, 1.0), (w_down.data_ptr(), None, 1.0)
-        api._check(api.library().b200_moe_layer(
+    if four_bit:
+        _require_cuda(w_gate_up.device, "w_gate_up", device)
+        _require_cuda(w_down.device, "w_down", device)
+        w1 = (FORMATS[w_gate_up.format], w_gate_up._data_ptr, w_gate_up._scales_ptr, w_gate_up.tensor_scale)
+        w2 = (w_down._data_ptr, w_down._scales_ptr, w_down.tensor_scale)
+    else:
+        w1, w2 = (-1, w_gate_up.data_ptr(), None, 1.0), (w_down.data_ptr(), None, 1.0)
+
+    def body(handle):
+        y = out if out is not None else torch.empty((T, H), dtype=x.dtype, device=device)
+        ws = workspace if workspace is not None else torch.empty(need, dtype=torch.uint8, device=device)
+        ids = torch.empty((T, top_k), dtype=torch.int32, device=device) if return_routing else None
+        weights = torch.empty((T, top_k), dtype=torch.float32, device=device) if return_routing else None
+        rc = api.library().b200_moe_layer(
             f16, T, E, top_k, H, I, x.data_ptr(), router.data_ptr(), bias.data_ptr() if bias is not None else None, *w1,
-            *w2, int(bool(renormalize)), out.data_ptr(), ids.data_ptr() if ids is not None else None,
-            weights.data_ptr() if weights is not None else None, workspace.data_ptr(), nbytes, s))
-    return (out, ids, weights) if return_routing else out
+            *w2, 1 if renormalize else 0, y.data_ptr(), ids.data_ptr() if return_routing else None,
+            weights.data_ptr() if return_routing else None, ws.data_ptr(), need, handle)
+        if rc:
+            api._check(rc)
+        return (y, ids, weights) if return_routing else y
+
+    return _run(device, stream, body)

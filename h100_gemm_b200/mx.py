@@ -17,9 +17,7 @@ blocks have to run along the contraction::
 from __future__ import annotations
 
 import contextlib
-import ctypes
 import math
-from dataclasses import dataclass
 
 from . import api
 from .api import STATUS_INVALID_ARG, GemmError
@@ -34,48 +32,81 @@ def _invalid(message: str) -> GemmError:
 
 
 def _format(name) -> int:
-    if name not in FORMATS:
+    fmt = FORMATS.get(name)
+    if fmt is None:
         raise _invalid(f"format must be one of {sorted(FORMATS)}, got {name!r}")
-    return FORMATS[name]
+    return fmt
 
 
-@dataclass
+def _pitch(cols: int) -> int:
+    """b200_mx_data_bytes of one row."""
+    return ((cols + 1) // 2 + 15) // 16 * 16
+
+
+def _scale_bytes(format: str, rows: int, cols: int) -> int:
+    """b200_mx_scale_bytes."""
+    return ((rows + 127) // 128) * ((cols + 255) // 256) * (_GROUPS[format] * 512)
+
+
 class MxTensor:
     """A [rows, cols] matrix in microscaled 4-bit form: ``data`` [rows, pitch] and ``scales`` [bytes],
     both uint8 CUDA tensors in the layout of include/b200_gemm.h. ``tensor_scale`` is the power of two
     (any positive number for matrices that come from elsewhere) all values are multiplied with."""
-    data: object
-    scales: object
-    rows: int
-    cols: int
-    format: str = "mxfp4"
-    tensor_scale: float = 1.0
 
-    def __post_init__(self):
+    __slots__ = ("rows", "cols", "format", "tensor_scale", "device", "_data", "_scales", "_pool", "_data_ptr", "_scales_ptr")
+
+    def __init__(self, data, scales, rows: int, cols: int, format: str = "mxfp4", tensor_scale: float = 1.0):
         import torch
-        fmt = _format(self.format)
-        lib = api.library()
-        if self.rows <= 0 or self.cols <= 0:
+        _format(format)
+        if rows <= 0 or cols <= 0:
             raise _invalid("rows and cols must be positive")
-        for name, t, need in (("data", self.data, lib.b200_mx_data_bytes(self.rows, self.cols)),
-                              ("scales", self.scales, lib.b200_mx_scale_bytes(fmt, self.rows, self.cols))):
-            if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or not t.is_contiguous():
+        if not (tensor_scale > 0 and math.isfinite(tensor_scale)):
+            raise _invalid("tensor_scale must be positive and finite")
+        if format == "mxfp4" and tensor_scale != 1.0:
+            raise _invalid("mxfp4 has no tensor scale (it must be 1)")
+        pointers = []
+        for name, t, need in (("data", data, rows * _pitch(cols)), ("scales", scales, _scale_bytes(format, rows, cols))):
+            if not isinstance(t, torch.Tensor) or t.dtype is not torch.uint8 or not t.is_contiguous():
                 raise _invalid(f"{name} must be a contiguous uint8 tensor")
             if t.numel() != need:
-                raise _invalid(f"{name} must hold {need} bytes for [{self.rows}, {self.cols}] {self.format}, "
-                               f"got {t.numel()}")
-            if t.data_ptr() % 16:
+                raise _invalid(f"{name} must hold {need} bytes for [{rows}, {cols}] {format}, got {t.numel()}")
+            pointers.append(t.data_ptr())
+            if pointers[-1] % 16:
                 raise _invalid(f"{name} must start on 16 bytes")
-        if self.data.device != self.scales.device:
+        if data.device != scales.device:
             raise _invalid("data and scales must be on one device")
-        if not (self.tensor_scale > 0 and math.isfinite(self.tensor_scale)):
-            raise _invalid("tensor_scale must be positive and finite")
-        if self.format == "mxfp4" and self.tensor_scale != 1.0:
-            raise _invalid("mxfp4 has no tensor scale (it must be 1)")
+        self.rows, self.cols, self.format, self.tensor_scale, self.device = rows, cols, format, tensor_scale, data.device
+        self._data, self._scales, self._pool = data, scales, None
+        self._data_ptr, self._scales_ptr = pointers
+
+    @classmethod
+    def _empty(cls, rows: int, cols: int, format: str, tensor_scale: float, device) -> "MxTensor":
+        """Uninitialised, in one allocation; the two tensors are made when somebody asks for them."""
+        import torch
+        self = cls.__new__(cls)
+        codes = rows * _pitch(cols)
+        at = (codes + 255) // 256 * 256
+        self._pool = torch.empty(at + _scale_bytes(format, rows, cols), dtype=torch.uint8, device=device)
+        self.rows, self.cols, self.format, self.tensor_scale, self.device = rows, cols, format, tensor_scale, device
+        self._data = self._scales = None
+        self._data_ptr = self._pool.data_ptr()
+        self._scales_ptr = self._data_ptr + at
+        return self
 
     @property
-    def device(self):
-        return self.data.device
+    def data(self):
+        if self._data is None:
+            self._data = self._pool[:self.rows * _pitch(self.cols)].view(self.rows, -1)
+        return self._data
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            self._scales = self._pool[self._scales_ptr - self._data_ptr:]
+        return self._scales
+
+    def __repr__(self):
+        return f"MxTensor([{self.rows}, {self.cols}], {self.format}, tensor_scale={self.tensor_scale}, device={self.device})"
 
     @classmethod
     def from_parts(cls, codes, block_scales, cols: int, format: str = "mxfp4", tensor_scale: float = 1.0) -> "MxTensor":
@@ -83,16 +114,15 @@ class MxTensor:
         [rows, ceil(cols / block)] (uint8 or the 8-bit float's own type), once."""
         import torch
         _format(format)
-        rows = codes.shape[0]
         blocks = -(-cols // BLOCK[format])
         if codes.dim() != 2 or block_scales.dim() != 2 or codes.shape[1] != (cols + 1) // 2 or \
-                tuple(block_scales.shape) != (rows, blocks):
+                tuple(block_scales.shape) != (codes.shape[0], blocks):
             raise _invalid(f"codes must be [rows, {(cols + 1) // 2}] and block_scales [rows, {blocks}]")
         if codes.element_size() != 1 or block_scales.element_size() != 1:
             raise _invalid("codes and block_scales must be 8-bit tensors")
+        rows = codes.shape[0]
         codes, block_scales = codes.view(torch.uint8), block_scales.view(torch.uint8)
-        pitch = ((cols + 1) // 2 + 15) // 16 * 16
-        data = torch.zeros(rows, pitch, dtype=torch.uint8, device=codes.device)
+        data = torch.zeros(rows, _pitch(cols), dtype=torch.uint8, device=codes.device)
         data[:, :codes.shape[1]] = codes
         if cols % 2:
             data[:, cols // 2] &= 15
@@ -111,9 +141,9 @@ class MxTensor:
 
 
 @contextlib.contextmanager
-def _on(device, stream):
-    """Runs a call on the tensors' device and, for memory it allocates, in the order of its stream; gives
-    the stream as the C ABI takes it."""
+def _elsewhere(device, stream):
+    """Another device than the current one, or a stream of the caller's choice: memory is allocated there, in
+    that stream's order."""
     import torch
     with torch.cuda.device(device):
         if stream is None:
@@ -124,57 +154,78 @@ def _on(device, stream):
             outer = torch.cuda.default_stream()
         else:
             outer = stream if isinstance(stream, torch.cuda.Stream) else torch.cuda.ExternalStream(handle)
-        if outer.device != torch.device(device):
-            raise _invalid(f"the stream belongs to {outer.device}, the tensors to {device}")
+        if getattr(stream, "device", outer.device) != device:
+            raise _invalid(f"the stream belongs to {stream.device}, the tensors to {device}")
         with torch.cuda.stream(outer):
             yield handle or None
 
 
-def _require_cuda(t, name: str, device=None):
-    if not t.is_cuda:
+def _run(device, stream, body):
+    """body(stream handle) on the tensors' device and stream; the usual case, the current ones, costs two lookups."""
+    import torch
+    if stream is None and torch.cuda.current_device() == device.index:
+        return body(torch._C._cuda_getCurrentRawStream(device.index) or None)
+    with _elsewhere(device, stream) as handle:
+        return body(handle)
+
+
+def _require_cuda(device, name: str, expected=None):
+    if device.type != "cuda":
         raise _invalid(f"{name} must be a CUDA tensor (no CPU fallback exists)")
-    if device is not None and t.device != device:
-        raise _invalid(f"{name} is on {t.device}, expected {device}")
+    if expected is not None and device != expected:
+        raise _invalid(f"{name} is on {device}, expected {expected}")
 
 
 def _half_type(dtype, name: str) -> int:
     import torch
-    if dtype not in (torch.bfloat16, torch.float16):
-        raise _invalid(f"{name} must be bfloat16 or float16, got {dtype}")
-    return int(dtype == torch.float16)
+    if dtype is torch.bfloat16:
+        return 0
+    if dtype is torch.float16:
+        return 1
+    raise _invalid(f"{name} must be bfloat16 or float16, got {dtype}")
 
 
-def _quantize(x, format, tensor_scale, out, out_t, rows: bool, cols: bool, stream):
-    import torch
+def _row_stride(t, name: str) -> int:
+    """Elements between the rows of a 2-D tensor whose columns are contiguous."""
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if cols > 1 and step != 1:
+        raise _invalid(f"the columns of {name} must be contiguous (its rows may be any distance apart)")
+    if rows == 1:
+        return cols
+    if ld < cols:
+        raise _invalid(f"the rows of {name} overlap")
+    return ld
+
+
+def _quantize(x, format, tensor_scale, out, rows: bool, cols: bool, stream):
     fmt = _format(format)
     f16 = _half_type(x.dtype, "x")
-    if x.dim() != 2 or x.shape[0] == 0 or x.shape[1] == 0:
+    if x.dim() != 2 or x.numel() == 0:
         raise _invalid("x must be a 2-D tensor with at least one row and one column")
-    if x.shape[1] > 1 and x.stride(1) != 1:
-        raise _invalid("the columns of x must be contiguous (its rows may be any distance apart)")
     R, C = x.shape
-    ld = x.stride(0) if R > 1 else C
-    if ld < C:
-        raise _invalid("the rows of x overlap")
-    _require_cuda(x, "x")
-    with _on(x.device, stream) as s:
-        lib = api.library()
+    ld = _row_stride(x, "x")
+    device = x.device
+    _require_cuda(device, "x")
+    if format == "mxfp4" and tensor_scale != 1.0:
+        raise _invalid("mxfp4 has no tensor scale (it must be 1)")
+    if out is not None:
+        want = (R, C) if rows else (C, R)
+        if (out.rows, out.cols) != want or out.format != format or out.tensor_scale != tensor_scale:
+            raise _invalid(f"out must be a [{want[0]}, {want[1]}] {format} matrix with tensor scale {tensor_scale}")
+        _require_cuda(out.device, "out", device)
 
-        def target(given, r, c, name):
-            if given is None:
-                data = torch.empty((r, lib.b200_mx_data_bytes(1, c)), dtype=torch.uint8, device=x.device)
-                scales = torch.empty(lib.b200_mx_scale_bytes(fmt, r, c), dtype=torch.uint8, device=x.device)
-                return MxTensor(data, scales, r, c, format, tensor_scale)
-            if (given.rows, given.cols, given.format) != (r, c, format) or given.tensor_scale != tensor_scale:
-                raise _invalid(f"{name} must be a [{r}, {c}] {format} matrix with tensor scale {tensor_scale}")
-            _require_cuda(given.data, name, x.device)
-            return given
+    def body(handle):
+        q = (out or MxTensor._empty(R, C, format, tensor_scale, device)) if rows else None
+        qt = (out or MxTensor._empty(C, R, format, tensor_scale, device)) if cols else None
+        rc = api.library().b200_mx_quantize(
+            fmt, f16, R, C, x.data_ptr(), ld, tensor_scale, q._data_ptr if rows else None, q._scales_ptr if rows else None,
+            qt._data_ptr if cols else None, qt._scales_ptr if cols else None, handle)
+        if rc:
+            api._check(rc)
+        return q, qt
 
-        q = target(out, R, C, "out") if rows else None
-        qt = target(out_t, C, R, "out") if cols else None
-        ptr = lambda m: (m.data.data_ptr(), m.scales.data_ptr()) if m is not None else (None, None)  # noqa: E731
-        api._check(lib.b200_mx_quantize(fmt, f16, R, C, x.data_ptr(), ld, tensor_scale, *ptr(q), *ptr(qt), s))
-    return q, qt
+    return _run(device, stream, body)
 
 
 def quantize_mx(x, format: str = "mxfp4", transpose: bool = False, tensor_scale: float = 1.0, out=None,
@@ -183,13 +234,19 @@ def quantize_mx(x, format: str = "mxfp4", transpose: bool = False, tensor_scale:
     ``transpose`` the 4-bit form of its transpose [C, R]. ``tensor_scale`` (nvfp4): a power of two near
     the matrix' largest magnitude / 2688, or 1 for values of ordinary size; block scales below 2^-9 of
     it are lost. ``out`` takes an MxTensor of the same shape and format to write into."""
-    q, qt = _quantize(x, format, tensor_scale, out, out, not transpose, transpose, stream)
+    q, qt = _quantize(x, format, tensor_scale, out, not transpose, transpose, stream)
     return qt if transpose else q
 
 
 def quantize_mx_both(x, format: str = "mxfp4", tensor_scale: float = 1.0, stream=None):
     """``(quantize_mx(x), quantize_mx(x, transpose=True))`` in one pass over x."""
-    return _quantize(x, format, tensor_scale, None, None, True, True, stream)
+    return _quantize(x, format, tensor_scale, None, True, True, stream)
+
+
+def _output(out, shape, dtype, device, contiguous: bool) -> None:
+    _require_cuda(out.device, "out", device)
+    if out.dtype is not dtype or tuple(out.shape) != shape or (contiguous and not out.is_contiguous()):
+        raise _invalid(f"out must be a {'contiguous ' if contiguous else ''}{list(shape)} {dtype} tensor")
 
 
 def dequantize_mx(q: MxTensor, dtype=None, out=None, stream=None):
@@ -197,19 +254,21 @@ def dequantize_mx(q: MxTensor, dtype=None, out=None, stream=None):
     import torch
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
     f16 = _half_type(dtype, "dtype")
-    _require_cuda(q.data, "q")
-    with _on(q.device, stream) as s:
-        if out is None:
-            out = torch.empty((q.rows, q.cols), dtype=dtype, device=q.device)
-        _require_cuda(out, "out", q.device)
-        if out.dtype != dtype or tuple(out.shape) != (q.rows, q.cols) or (q.cols > 1 and out.stride(1) != 1):
-            raise _invalid(f"out must be a [{q.rows}, {q.cols}] {dtype} tensor with contiguous columns")
-        ld = out.stride(0) if q.rows > 1 else q.cols
-        if ld < q.cols:
-            raise _invalid("the rows of out overlap")
-        api._check(api.library().b200_mx_dequantize(_format(q.format), f16, q.rows, q.cols, q.data.data_ptr(),
-                                                    q.scales.data_ptr(), q.tensor_scale, out.data_ptr(), ld, s))
-    return out
+    device, shape = q.device, (q.rows, q.cols)
+    _require_cuda(device, "q")
+    if out is not None:
+        _output(out, shape, dtype, device, False)
+
+    def body(handle):
+        y = out if out is not None else torch.empty(shape, dtype=dtype, device=device)
+        rc = api.library().b200_mx_dequantize(FORMATS[q.format], f16, q.rows, q.cols, q._data_ptr, q._scales_ptr,
+                                              q.tensor_scale, y.data_ptr(), q.cols if out is None else _row_stride(out, "out"),
+                                              handle)
+        if rc:
+            api._check(rc)
+        return y
+
+    return _run(device, stream, body)
 
 
 def gemm_mx(a: MxTensor, b: MxTensor, out=None, alpha: float = 1.0, beta: float = 0.0, dtype=None, stream=None):
@@ -222,16 +281,18 @@ def gemm_mx(a: MxTensor, b: MxTensor, out=None, alpha: float = 1.0, beta: float 
         raise _invalid(f"a is {a.format}, b is {b.format}")
     if a.cols != b.cols:
         raise _invalid("a and b disagree on K")
-    _require_cuda(a.data, "a")
-    _require_cuda(b.data, "b", a.device)
-    scale = float(alpha) * a.tensor_scale * b.tensor_scale
-    with _on(a.device, stream) as s:
-        if out is None:
-            out = torch.empty((a.rows, b.rows), dtype=dtype, device=a.device)
-        _require_cuda(out, "out", a.device)
-        if out.dtype != dtype or tuple(out.shape) != (a.rows, b.rows) or not out.is_contiguous():
-            raise _invalid(f"out must be a contiguous [{a.rows}, {b.rows}] {dtype} tensor")
-        api._check(api.library().b200_gemm_mx(_format(a.format), f16, a.rows, b.rows, a.cols, a.data.data_ptr(),
-                                              a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(),
-                                              out.data_ptr(), scale, beta, s))
-    return out
+    device, shape = a.device, (a.rows, b.rows)
+    _require_cuda(device, "a")
+    _require_cuda(b.device, "b", device)
+    if out is not None:
+        _output(out, shape, dtype, device, True)
+
+    def body(handle):
+        c = out if out is not None else torch.empty(shape, dtype=dtype, device=device)
+        rc = api.library().b200_gemm_mx(FORMATS[a.format], f16, a.rows, b.rows, a.cols, a._data_ptr, a._scales_ptr, b._data_ptr,
+                                        b._scales_ptr, c.data_ptr(), alpha * a.tensor_scale * b.tensor_scale, beta, handle)
+        if rc:
+            api._check(rc)
+        return c
+
+    return _run(device, stream, body)
