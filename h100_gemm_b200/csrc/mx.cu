@@ -103,46 +103,99 @@ struct MxProduct {
   const void *x, *sx, *w, *sw;
 };
 
-template <int FMT, int BN, int F16>
-int launch_gemm(const DeviceInfo& dev, const MxProduct& p, MxGemmArgs args, cudaStream_t stream) {
-  using T = MxGemmTraits<FMT, BN>;
-  args.tiles_r = static_cast<int>(mx_row_tiles(p.R));
+// How a product is cut: CTAs of 128 x BN or pairs of 256 x BN, and the K ranges that share a tile.
+struct MxPlan {
+  int width;       // BN
+  int pair;
+  int transposed;
+  int split;
+};
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+// The cut by shape. Up to 64 rows of A ride on the MMA's N in the narrowest tile that holds them, and 128 weight
+// rows per CTA: two CTAs per SM, so that up to 296 tiles stream at a time. Beyond, CTA pairs: 256 weight
+// rows against 128 or 256 rows of A while that leaves pairs idle (then K is shared out), else 256
+// rows of A against 256 weight rows, row-major.
+MxPlan plan_product(int M, int N, int K, int sms) {
+  const long long k_tiles = mx_col_tiles(K);
+  MxPlan p{};
+  p.transposed = 1;
+  p.split = 1;
+  if (M <= 64) {
+    p.width = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    const long long tiles = ceil_div(N, 128);
+    while (p.split < 8 && tiles * (p.split + 1) <= 2ll * sms && k_tiles >= 4ll * (p.split + 1)) ++p.split;
+    return p;
+  }
+  p.pair = 1;
+  p.width = M <= 128 ? 128 : 256;
+  const long long tiles = ceil_div(N, 256) * ceil_div(M, p.width);
+  while (p.split < 4 && tiles * (p.split + 1) <= sms / 2 && k_tiles >= 4ll * (p.split + 1)) ++p.split;
+  if (p.split == 1 && M > 256) p.transposed = 0;
+  return p;
+}
+
+template <int FMT, int BN, int PAIR, int F16>
+int launch_gemm(const DeviceInfo& dev, const MxProduct& p, const MxPlan& plan, MxGemmArgs args, cudaStream_t stream) {
+  using T = MxGemmTraits<FMT, BN, PAIR>;
   args.k_tiles = static_cast<int>(mx_col_tiles(p.K));
-  const long long tiles = static_cast<long long>(args.tiles_r) * ((p.S + BN - 1) / BN);
-  // Two CTAs to an SM where their rings and accumulators fit: 113 KB of shared memory and half of
-  // tensor memory each.
-  const bool two = T::smem_bytes(kMxScaleBuffers) <= 113 * 1024 && T::kTmemCols <= 256;
-  const long long slots = static_cast<long long>(dev.sm_count) * (two ? 2 : 1);
-  int split = 1;
-  while (split < 8 && tiles * split * 2 <= slots && args.k_tiles >= split * 2 * 4) split *= 2;
+  args.split = plan.split;
+  args.slab_bytes = plan.transposed ? 0 : kMxSlabs * kMxSlabBytes;
+  args.sched.tiles_m = static_cast<int>(ceil_div(p.R, T::kTileRows));
+  args.sched.tiles_n = static_cast<int>(ceil_div(p.S, BN));
+  args.sched.batch = 1;
+  const long long tiles = static_cast<long long>(args.sched.tiles_m) * args.sched.tiles_n;
+  if (tiles > 0x7FFFFFFFll / 16) return B200_ERR_INVALID_ARG;
+  args.sched.num_tiles = static_cast<int>(tiles);
+  args.sched.k_tiles = args.k_tiles;
+  args.sched.group = 8;
+  args.sched.mode = kDataParallel;
+  args.sched.split_k = 1;
+  // Two lone CTAs to an SM where their rings and accumulators fit: 113 KB of shared memory and half of tensor
+  // memory each.
+  const bool two = !PAIR && T::kTmemCols <= 256;
+  const long long workers = static_cast<long long>(dev.sm_count) * (two ? 2 : 1) / T::kCtas;
+  const long long waves = ceil_div(tiles, workers);
+  args.sched.num_workers = static_cast<int>(plan.split > 1 ? tiles : ceil_div(tiles, waves));
   const int budget = two ? 113 * 1024 : dev.smem_optin;
-  int stages = (budget - T::smem_bytes(0)) / T::kStageBytes;
+  int stages = (budget - T::smem_bytes(0, args.slab_bytes)) / T::kStageBytes;
   if (stages > kMxMaxStages) stages = kMxMaxStages;
-  if (stages < kMxScaleBuffers) return B200_ERR_SMEM;
+  if (stages < T::kScaleBuffers || (plan.split > 1 && stages * T::kStageBytes < BN * 512)) return B200_ERR_SMEM;
   args.stages = stages;
-  CUtensorMap mx, mw, msx, msw;
+  CUtensorMap mx, mw, msx, msw, mc;
   int rc = code_map(dev, &mx, p.x, p.R, p.K, 128);
-  if (rc == B200_OK) rc = code_map(dev, &mw, p.w, p.S, p.K, BN);
+  if (rc == B200_OK) rc = code_map(dev, &mw, p.w, p.S, p.K, T::kWRows);
   if (rc == B200_OK) rc = scale_map(dev, &msx, FMT, p.sx, p.R, p.K);
   if (rc == B200_OK) rc = scale_map(dev, &msw, FMT, p.sw, p.S, p.K);
   if (rc != B200_OK) return rc;
-  const auto kernel = &mx_gemm_kernel<FMT, BN, F16>;
+  args.tma_store = !plan.transposed && aligned16(args.C) && args.ldc % 8 == 0 ? 1 : 0;
+  if (args.tma_store) {
+    rc = tile_map(dev, &mc, CU_TENSOR_MAP_DATA_TYPE_UINT16, args.C, static_cast<uint64_t>(p.S), static_cast<uint64_t>(p.R),
+                  static_cast<uint64_t>(args.ldc) * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+    if (rc != B200_OK) return rc;
+  } else {
+    mc = mx;  // never followed
+  }
+  const auto kernel = &mx_gemm_kernel<FMT, BN, PAIR, F16>;
   static std::atomic<bool> allowed[64];
   rc = allow_shared_memory(dev, kernel, allowed);
   if (rc != B200_OK) return rc;
-  Launch l(tiles * split, T::kThreads, static_cast<size_t>(T::smem_bytes(stages)), stream, split);
-  B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, kernel, mx, mw, msx, msw, args, split));
+  const int cluster = plan.split * T::kCtas;
+  Launch l(static_cast<long long>(args.sched.num_workers) * cluster, T::kThreads,
+           static_cast<size_t>(T::smem_bytes(stages, args.slab_bytes)), stream, cluster);
+  B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, kernel, mx, mw, msx, msw, mc, args));
   return B200_OK;
 }
 
 template <int FMT, int F16>
-int launch_gemm(const DeviceInfo& dev, const MxProduct& p, const MxGemmArgs& args, int width, cudaStream_t stream) {
-  switch (width) {
-    case 16: return launch_gemm<FMT, 16, F16>(dev, p, args, stream);
-    case 32: return launch_gemm<FMT, 32, F16>(dev, p, args, stream);
-    case 64: return launch_gemm<FMT, 64, F16>(dev, p, args, stream);
-    case 128: return launch_gemm<FMT, 128, F16>(dev, p, args, stream);
-    default: return launch_gemm<FMT, 256, F16>(dev, p, args, stream);
+int launch_gemm(const DeviceInfo& dev, const MxProduct& p, const MxPlan& plan, const MxGemmArgs& args, cudaStream_t stream) {
+  switch (plan.width) {
+    case 16: return launch_gemm<FMT, 16, 0, F16>(dev, p, plan, args, stream);
+    case 32: return launch_gemm<FMT, 32, 0, F16>(dev, p, plan, args, stream);
+    case 64: return launch_gemm<FMT, 64, 0, F16>(dev, p, plan, args, stream);
+    case 128: return launch_gemm<FMT, 128, 1, F16>(dev, p, plan, args, stream);
+    default: return launch_gemm<FMT, 256, 1, F16>(dev, p, plan, args, stream);
   }
 }
 
@@ -239,33 +292,29 @@ int b200_gemm_mx(int format, int f16, int M, int N, int K, const void* A, const 
   DeviceInfo dev;
   const int rc = device_info(&dev);
   if (rc != B200_OK) return rc;
-  // Up to 128 rows ride on the MMA's N, in the narrowest tile that holds them, and C is stored
-  // transposed; with more rows A takes the MMA's M.
-  const bool few = M <= 128;
+  const MxPlan plan = plan_product(M, N, K, dev.sm_count);
   MxProduct p;
   MxGemmArgs args;
   std::memset(&args, 0, sizeof args);
-  if (few) {
+  if (plan.transposed) {
     p = MxProduct{N, M, K, B, B_scales, A, A_scales};
   } else {
     p = MxProduct{M, N, K, A, A_scales, B, B_scales};
   }
   args.R = p.R;
   args.S = p.S;
-  args.transposed = few ? 1 : 0;
-  args.vec = !few && aligned16(C) && N % 8 == 0 ? 1 : 0;
+  args.transposed = plan.transposed;
   args.C = static_cast<uint16_t*>(C);
   args.ldc = N;
   args.alpha = alpha;
   args.beta = beta;
   args.scale = (alpha != 1.0f || beta != 0.0f) ? 1 : 0;
   args.status = dev.status;
-  const int width = few ? (M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128) : (N <= 128 ? 128 : 256);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (format == B200_MXFP4) {
-    return f16 ? launch_gemm<kMxfp4, 1>(dev, p, args, width, s) : launch_gemm<kMxfp4, 0>(dev, p, args, width, s);
+    return f16 ? launch_gemm<kMxfp4, 1>(dev, p, plan, args, s) : launch_gemm<kMxfp4, 0>(dev, p, plan, args, s);
   }
-  return f16 ? launch_gemm<kNvfp4, 1>(dev, p, args, width, s) : launch_gemm<kNvfp4, 0>(dev, p, args, width, s);
+  return f16 ? launch_gemm<kNvfp4, 1>(dev, p, plan, args, s) : launch_gemm<kNvfp4, 0>(dev, p, plan, args, s);
 }
 
 }  // extern "C"

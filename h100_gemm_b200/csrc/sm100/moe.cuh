@@ -438,17 +438,6 @@ struct MoeUnit {
   static constexpr float kLift = W == kMoeNvfp4 ? kNvfp4Lift : 1.0f;
 };
 
-// Joins the eight warps' accumulators (and those of the other CTAs of a cluster) in order: the sum of
-// element `idx` (one lane's four values of one tile).
-B200_DEVICE float4 ld_cluster_v4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
-}
-
 B200_DEVICE float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 
 // ------------------------------------------------------------------------------------- gate and up
@@ -601,7 +590,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_c
     for (int p = 0; p < split; ++p) {
       const uint32_t base = split > 1 ? ptx::map_to_cta(red_addr, static_cast<uint32_t>(p)) : red_addr;
       for (int q = 0; q < kMoeWarps; ++q) {
-        const float4 v = ld_cluster_v4(base + static_cast<uint32_t>((q * MT * NT * 32 + idx) * 16));
+        const float4 v = ptx::ld_cluster_v4(base + static_cast<uint32_t>((q * MT * NT * 32 + idx) * 16));
         s.x += v.x;
         s.y += v.y;
         s.z += v.z;

@@ -9,57 +9,83 @@
 // tcgen05.cp moves them to tensor memory unchanged.
 //
 //   warp 0      TMA producer: codes and scales of both operands into a shared-memory ring
-//   warp 1      MMA issuer: scales to tensor memory, four MMAs of K = 64 per K-tile
-//   warps 2-5   epilogue: accumulator -> registers -> C
+//   warp 1      MMA issuer: four MMAs of K = 64 per K-tile
+//   warp 2      scale copies: shared -> tensor memory, ahead of the MMAs
+//   warps 3-6   epilogue: accumulator -> registers -> C
 //
-// One CTA computes a 128 x BN tile, X's rows on the MMA's M. With few rows in the caller's A the operands are
-// swapped (C is written transposed): weights on M, the rows on N, so that no tensor work and no
-// accumulator is spent on padding. When there are fewer tiles than SMs a cluster of CTAs shares one
-// tile, each taking a range of K; the partial tiles are added over distributed shared memory in rank order, so that
-// no workspace is needed, nothing depends on timing and a captured launch can be replayed.
+// X's rows ride on the MMA's M (128 per CTA), W's on its N (BN per tile). PAIR = 1 drives two CTAs with one
+// cta_group::2 MMA: 256 x BN, each CTA staging its own rows of X and half of W's. Feeding these
+// MMAs is what limits a large product: a K-tile of a lone 128 x 256 tile takes 540 cycles at the nominal rate and
+// 51 KB of loads, 94 bytes per cycle and SM; a pair loads 35 KB for the same work.
+//
+// C is X W^T row-major (A is X), or its transpose (the weights are X: `transposed`). The transposed form
+// serves few rows, so that no tensor work and no accumulator is spent on padding, and everything that
+// is short of tiles: there a cluster of CTAs (pairs) shares one tile, each taking a range of K, and the
+// partial tiles are added over distributed shared memory in rank order. No workspace is needed, nothing depends on
+// timing and a captured launch can be replayed.
+//
+// Tensor memory (512 columns): two accumulators, and the scales of the last kScaleBuffers K-tiles. With
+// BN = 256 the accumulators overlap by the columns the scales need: the epilogue reads those first and
+// hands them back before the rest, so all the next tile waits for is that part of the read-out.
 #pragma once
 
 #include "desc.cuh"
 #include "mx_format.cuh"
 #include "ptx.cuh"
+#include "scheduler.cuh"
 #include "status.cuh"
 
 namespace b200 {
 
 struct MxGemmArgs {
-  int R, S;           // rows of X and W
-  int k_tiles;        // K-tiles of 256 elements
-  int tiles_r;        // tiles along R
+  int R, S;            // rows of X and W
+  int k_tiles;         // K-tiles of 256 elements
+  SchedParams sched;   // whole tiles in raster order
+  int split;           // CTAs (pairs) that share a tile; above 1 every cluster has one tile
   int stages;
-  int transposed;     // 1: element (r, s) goes to C[s * ldc + r]
-  int vec;            // 1: rows of C start on 16 bytes and S is a multiple of 8
+  int transposed;      // 1: element (r, s) goes to C[s * ldc + r]
+  int tma_store;       // 1: rows of C start on 16 bytes and S is a multiple of 8 (row-major only)
+  int slab_bytes;      // epilogue staging per warp (row-major only)
   uint16_t* C;
   long long ldc;
   float alpha, beta;
-  int scale;          // 1: C = acc * alpha + beta
+  int scale;           // 1: C = acc * alpha + beta
   unsigned int* status;
 };
 
 static constexpr int kMxMaxStages = 16;
-static constexpr int kMxScaleBuffers = 3;  // K-tiles whose scales tensor memory holds at a time (the ring has no fewer stages)
+static constexpr int kMxSlabBytes = 32 * 64;  // 32 rows x 32 columns of 16-bit output
+static constexpr int kMxSlabs = 2;            // per epilogue warp
 
-template <int FMT, int BN>
+template <int FMT, int BN, int PAIR>
 struct MxGemmTraits {
-  static constexpr int kThreads = 192;
+  static constexpr int kThreads = 224;
+  static constexpr int kCtas = PAIR ? 2 : 1;
+  static constexpr int kTileRows = 128 * kCtas;
   static constexpr int kSBlocks = (BN + 127) / 128;                 // scale tiles of W per K-tile
   static constexpr int kXBytes = 128 * 128;
-  static constexpr int kWBytes = BN * 128;
+  static constexpr int kWRows = BN / kCtas;                         // staged by one CTA
+  static constexpr int kWBytes = kWRows * 128;
   static constexpr int kScaleTile = mx_tile_bytes(FMT);
   static constexpr int kGroups = mx_tile_groups(FMT);
   static constexpr int kStageBytes = kXBytes + kWBytes + (1 + kSBlocks) * kScaleTile;
-  static constexpr int kAccCols = BN < 32 ? 32 : BN;
   static constexpr int kScaleCols = kGroups * 4 * (1 + kSBlocks);   // of one K-tile: X's, then W's
-  static constexpr int kNeedCols = kAccCols + kMxScaleBuffers * kScaleCols;
+  // K-tiles whose scales tensor memory holds; never more than the ring has stages. NVFP4 has twice the scales: three
+  // where tensor memory (BN = 256) or half an SM's shared memory (BN = 64) has no room for a fourth.
+  static constexpr int kScaleBuffers = FMT == kNvfp4 && (BN == 256 || BN == 64) ? 3 : 4;
+  static constexpr int kScalesNeed = kScaleBuffers * kScaleCols;
+  static constexpr int kAccCols = BN < 32 ? 32 : BN;
+  // Columns the two accumulators share, in whole 32-column reads.
+  static constexpr int kOverlap = 2 * kAccCols + kScalesNeed > 512 ? (2 * kAccCols + kScalesNeed - 512 + 31) / 32 * 32 : 0;
+  static constexpr int kAcc1 = kAccCols - kOverlap;                 // first column of the second accumulator
+  static constexpr int kScales0 = kAcc1 + kAccCols;
+  static constexpr int kNeedCols = kScales0 + kScalesNeed;
   static constexpr int kTmemCols = kNeedCols <= 128 ? 128 : kNeedCols <= 256 ? 256 : 512;
-  static_assert(kNeedCols <= 512, "accumulator and scales exceed tensor memory");
-  static_assert(BN % 16 == 0 && BN <= 256, "width of the MMA");
+  static_assert(kNeedCols <= 512, "accumulators and scales exceed tensor memory");
+  static_assert(BN % 16 == 0 && BN <= 256 && (!PAIR || BN >= 64), "width of the MMA");
+  static_assert(kWBytes % 1024 == 0, "swizzled tiles start on 1024 bytes");
   static constexpr int kBarrierBytes = 512;
-  static constexpr int smem_bytes(int stages) { return 1024 + stages * kStageBytes + kBarrierBytes; }
+  static constexpr int smem_bytes(int stages, int slabs) { return 1024 + stages * kStageBytes + 4 * slabs + kBarrierBytes; }
 };
 
 __device__ __forceinline__ void mx_report_timeout(unsigned int* status, unsigned int code, int tile, int detail,
@@ -87,229 +113,410 @@ __device__ __forceinline__ float mx_finish(const MxGemmArgs& args, float acc) {
   return args.scale ? __fadd_rn(__fmul_rn(acc, args.alpha), args.beta) : acc;
 }
 
-// Grid: tiles * split CTAs, clusters of `split`; CTA rank r of a cluster takes K-tiles
-// [k_tiles * r / split, k_tiles * (r + 1) / split).
-template <int FMT, int BN, int F16>
-__global__ void __launch_bounds__(192) mx_gemm_kernel(const __grid_constant__ CUtensorMap map_x,
+// Grid: clusters of split * (1 or 2) CTAs. Pair p of a cluster takes K-tiles
+// [k_tiles * p / split, k_tiles * (p + 1) / split) of each of the cluster's tiles.
+template <int FMT, int BN, int PAIR, int F16>
+__global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CUtensorMap map_x,
                                                        const __grid_constant__ CUtensorMap map_w,
                                                        const __grid_constant__ CUtensorMap map_sx,
                                                        const __grid_constant__ CUtensorMap map_sw,
-                                                       const __grid_constant__ MxGemmArgs args, int split) {
-  using T = MxGemmTraits<FMT, BN>;
+                                                       const __grid_constant__ CUtensorMap map_c,
+                                                       const __grid_constant__ MxGemmArgs args) {
+  using T = MxGemmTraits<FMT, BN, PAIR>;
+  constexpr int G = T::kCtas;
   extern __shared__ uint8_t smem_raw[];
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x) / 32, 0);
   const uint32_t lane = ptx::lane_id();
-  const int rank = split > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
-  const int tile = static_cast<int>(blockIdx.x) / split;
-  const int r0 = (tile % args.tiles_r) * 128;
-  const int s0 = (tile / args.tiles_r) * BN;
-  const int kt0 = static_cast<int>(static_cast<long long>(args.k_tiles) * rank / split);
-  const int kt1 = static_cast<int>(static_cast<long long>(args.k_tiles) * (rank + 1) / split);
+  const int cluster_size = args.split * G;
+  const int cluster = static_cast<int>(blockIdx.x) / cluster_size;
+  const uint32_t cluster_rank = cluster_size > 1 ? ptx::cluster_ctarank() : 0u;
+  const uint32_t cta = PAIR ? cluster_rank & 1u : 0u;  // of the pair
+  const uint32_t leader = cluster_rank - cta;
+  const int part = static_cast<int>(cluster_rank) / G;
+  const int kt0 = static_cast<int>(static_cast<long long>(args.k_tiles) * part / args.split);
+  const int kt1 = static_cast<int>(static_cast<long long>(args.k_tiles) * (part + 1) / args.split);
 
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t bar_base = smem_base + static_cast<uint32_t>(args.stages * T::kStageBytes);
+  const uint32_t slab_base = smem_base + static_cast<uint32_t>(args.stages * T::kStageBytes);
+  const uint32_t bar_base = slab_base + static_cast<uint32_t>(4 * args.slab_bytes);
   auto stage_addr = [&](int s) { return smem_base + static_cast<uint32_t>(s * T::kStageBytes); };
   auto full_bar = [&](int s) { return bar_base + 8u * static_cast<uint32_t>(s); };
   auto empty_bar = [&](int s) { return bar_base + 8u * static_cast<uint32_t>(kMxMaxStages + s); };
-  const uint32_t done_bar = bar_base + 8u * (2 * kMxMaxStages);
-  const uint32_t tmem_slot = done_bar + 8u;
+  auto done_bar = [&](int a) { return bar_base + 8u * static_cast<uint32_t>(2 * kMxMaxStages + a); };
+  auto drained_bar = [&](int a) { return bar_base + 8u * static_cast<uint32_t>(2 * kMxMaxStages + 2 + a); };
+  auto scales_bar = [&](int b) { return bar_base + 8u * static_cast<uint32_t>(2 * kMxMaxStages + 4 + b); };
+  const uint32_t tmem_slot = bar_base + 8u * (2 * kMxMaxStages + 8);
   uint8_t* generic_bar = smem_raw + (bar_base - ptx::smem_u32(smem_raw));
-  volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(generic_bar + 8 * (2 * kMxMaxStages + 1));
+  volatile uint32_t* tmem_ptr = reinterpret_cast<volatile uint32_t*>(generic_bar + 8 * (2 * kMxMaxStages + 8));
   volatile uint32_t* abort_flag = tmem_ptr + 1;
 
-  ptx::grid_launch_dependents();
   if (warp == 0 && lane == 0) {
     ptx::prefetch_tensormap(&map_x);
     ptx::prefetch_tensormap(&map_w);
     ptx::prefetch_tensormap(&map_sx);
     ptx::prefetch_tensormap(&map_sw);
+    if (args.tma_store) ptx::prefetch_tensormap(&map_c);
     for (int s = 0; s < args.stages; ++s) {
       ptx::mbar_init(full_bar(s), 1);
       ptx::mbar_init(empty_bar(s), 1);
     }
-    ptx::mbar_init(done_bar, 1);
+    for (int a = 0; a < 2; ++a) {
+      ptx::mbar_init(done_bar(a), 1);
+      ptx::mbar_init(drained_bar(a), 4 * G);
+    }
+    for (int b = 0; b < T::kScaleBuffers; ++b) ptx::mbar_init(scales_bar(b), 1);
     *abort_flag = 0u;
     ptx::fence_mbar_init();
   }
   if (warp == 1) {
-    ptx::tmem_alloc<1>(tmem_slot, T::kTmemCols);
-    ptx::tmem_relinquish<1>();
+    ptx::tmem_alloc<G>(tmem_slot, T::kTmemCols);
+    ptx::tmem_relinquish<G>();
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
+  if (PAIR) {
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+  }
   ptx::tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_ptr;
+  ptx::grid_launch_dependents();  // (not before this CTA has its tensor memory: the next kernel's may wait for it)
   ptx::grid_dependency_wait();
 
   if (warp == 0) {
     if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      const int sx_tile = (r0 / kMxTileRows) * args.k_tiles, sw_tile = (s0 / kMxTileRows) * args.k_tiles;
+      const uint32_t leader_full = PAIR ? ptx::map_to_cta(full_bar(0), leader) : full_bar(0);
       constexpr int kBoxes = T::kScaleTile / 1024;  // 1 KB rows of the scale maps per tile
-      for (int kt = kt0; kt < kt1; ++kt) {
-        if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u)) {
-          mx_report_timeout(args.status, kStatusProducerTimeout, tile, kt, abort_flag);
-          break;
-        }
-        const uint32_t full = full_bar(stage), x = stage_addr(stage);
-        const uint32_t w = x + T::kXBytes, sx = w + T::kWBytes, sw = sx + T::kScaleTile;
-        ptx::mbar_arrive_expect_tx(full, T::kStageBytes);
-        ptx::tma_load_3d(x, &map_x, full, kt * 128, r0, 0);
-        ptx::tma_load_3d(w, &map_w, full, kt * 128, s0, 0);
-        ptx::tma_load_3d(sx, &map_sx, full, 0, (sx_tile + kt) * kBoxes, 0);
-#pragma unroll
-        for (int b = 0; b < T::kSBlocks; ++b) {
-          ptx::tma_load_3d(sw + b * T::kScaleTile, &map_sw, full, 0, (sw_tile + b * args.k_tiles + kt) * kBoxes, 0);
-        }
-        if (++stage == args.stages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    if (lane == 0) {
-      // 16-element blocks: every MMA has a scale column of its own; 32-element blocks: two MMAs share
-      // one, the second starting at its upper byte pair.
-      constexpr uint32_t idesc0 = make_instr_desc_mxf4(128, BN, FMT == kMxfp4, 0);
-      constexpr uint32_t idesc1 = make_instr_desc_mxf4(128, BN, FMT == kMxfp4, FMT == kMxfp4 ? 2 : 0);
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int kt = kt0; kt < kt1; ++kt) {
-        const int i = kt - kt0;
-        if (i >= kMxScaleBuffers) {
-          // The scales of K-tile i - kMxScaleBuffers are overwritten: its MMAs must have completed.
-          const int old = i - kMxScaleBuffers;
-          if (!ptx::mbar_wait(empty_bar(old % args.stages), static_cast<uint32_t>(old / args.stages) & 1u)) {
-            mx_report_timeout(args.status, kStatusMmaTmemTimeout, tile, kt, abort_flag);
+      for (int tile = cluster; ok && tile < args.sched.num_tiles; tile += args.sched.num_workers) {
+        const TileCoord tc = tile_coord(args.sched, tile);
+        const int r0 = tc.m * T::kTileRows + static_cast<int>(cta) * 128;
+        const int s0 = tc.n * BN;
+        const int w0 = s0 + static_cast<int>(cta) * T::kWRows;
+        const int sx_tile = (r0 / kMxTileRows) * args.k_tiles, sw_tile = (s0 / kMxTileRows) * args.k_tiles;
+        for (int kt = kt0; kt < kt1; ++kt) {
+          if (!ptx::mbar_wait(empty_bar(stage), phase ^ 1u)) {
+            mx_report_timeout(args.status, kStatusProducerTimeout, tile, kt, abort_flag);
             ok = false;
             break;
           }
+          const uint32_t full = leader_full + 8u * static_cast<uint32_t>(stage), x = stage_addr(stage);
+          const uint32_t w = x + T::kXBytes, sx = w + T::kWBytes, sw = sx + T::kScaleTile;
+          if (cta == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), T::kStageBytes * G);
+          auto load = [&](uint32_t dst, const CUtensorMap* map, int c0, int c1) {
+            if (PAIR) {
+              ptx::tma_load_3d_pair(dst, map, full, c0, c1, 0);
+            } else {
+              ptx::tma_load_3d(dst, map, full, c0, c1, 0);
+            }
+          };
+          load(x, &map_x, kt * 128, r0);
+          load(w, &map_w, kt * 128, w0);
+          load(sx, &map_sx, 0, (sx_tile + kt) * kBoxes);
+#pragma unroll
+          for (int b = 0; b < T::kSBlocks; ++b) {
+            load(sw + b * T::kScaleTile, &map_sw, 0, (sw_tile + b * args.k_tiles + kt) * kBoxes);
+          }
+          if (++stage == args.stages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp <= 2) {
+    const uint16_t both = static_cast<uint16_t>(3u << leader);
+    const int len = kt1 - kt0;
+    const int mine = args.sched.num_tiles > cluster ? (args.sched.num_tiles - cluster - 1) / args.sched.num_workers + 1 : 0;
+    if (warp == 1 && lane == 0 && cta == 0) {
+      // 16-element blocks: every MMA has a scale column of its own; 32-element blocks: two MMAs share
+      // one, the second starting at its upper byte pair.
+      constexpr uint32_t idesc0 = make_instr_desc_mxf4(T::kTileRows, BN, FMT == kMxfp4, 0);
+      constexpr uint32_t idesc1 = make_instr_desc_mxf4(T::kTileRows, BN, FMT == kMxfp4, FMT == kMxfp4 ? 2 : 0);
+      auto commit = [&](uint32_t bar) {
+        if (PAIR) {
+          ptx::umma_commit_pair(bar, both);
+        } else {
+          ptx::umma_commit_1cta(bar);
+        }
+      };
+      const uint64_t desc0 = make_smem_desc_sw128(smem_base);
+      uint64_t desc = desc0;
+      int stage = 0, buffer = 0;
+      uint32_t phase = 0, scales_phase = 0;
+      bool ok = true;
+      for (int turn = 0; ok && turn < mine; ++turn) {
+        // Overlapping accumulators: the tile before must have been read out where they overlap.
+        // Separate ones: the tile before that, entirely.
+        const bool wait_drained = T::kOverlap > 0 ? turn >= 1 : turn >= 2;
+        const uint32_t drained_phase = static_cast<uint32_t>(T::kOverlap > 0 ? turn - 1 : turn / 2 - 1) & 1u;
+        if (wait_drained && !ptx::mbar_wait(drained_bar(T::kOverlap > 0 ? 0 : turn & 1), drained_phase)) {
+          mx_report_timeout(args.status, kStatusMmaTmemTimeout, turn, 0, abort_flag);
+          break;
+        }
+        const uint32_t tmem_d = tmem_base + ((turn & 1) ? T::kAcc1 : 0);
+        for (int k_tile = 0; k_tile < len; ++k_tile) {
+          // (the copies were issued after the stage had landed, so the second wait only orders this thread)
+          if (!ptx::mbar_wait(scales_bar(buffer), scales_phase) || !ptx::mbar_wait(full_bar(stage), phase)) {
+            mx_report_timeout(args.status, kStatusMmaFullTimeout, turn, k_tile, abort_flag);
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after_sync();
+          const uint32_t tsx = tmem_base + T::kScales0 + static_cast<uint32_t>(buffer * T::kScaleCols);
+          const uint32_t tsw = tsx + T::kGroups * 4;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int g = FMT == kMxfp4 ? k / 2 : k;
+            ptx::umma_mxf4<G, FMT == kNvfp4>(tmem_d, desc + k * kDescKStep, desc + (T::kXBytes >> 4) + k * kDescKStep,
+                                             (k & 1) ? idesc1 : idesc0, tsx + g * 4, tsw + g * 4 * T::kSBlocks,
+                                             (k_tile > 0 || k > 0) ? 1u : 0u);
+          }
+          commit(empty_bar(stage));
+          desc += T::kStageBytes >> 4;
+          if (++stage == args.stages) {
+            stage = 0;
+            phase ^= 1u;
+            desc = desc0;
+          }
+          if (++buffer == T::kScaleBuffers) {
+            buffer = 0;
+            scales_phase ^= 1u;
+          }
+        }
+        if (ok) commit(done_bar(turn & 1));
+      }
+    } else if (warp == 2 && lane == 0 && cta == 0) {
+      const long long total = static_cast<long long>(mine) * len;  // K-tiles of all tiles, one sequence
+      const uint64_t desc0 = make_smem_desc_scales(smem_base + T::kXBytes + T::kWBytes);
+      uint64_t desc = desc0;
+      int stage = 0, buffer = 0, old_stage = 0;
+      uint32_t phase = 0, old_phase = 0;
+      for (long long i = 0; i < total; ++i) {
+        if (i >= T::kScaleBuffers) {
+          // What the buffer holds, the scales of the K-tile kScaleBuffers before, must have been used.
+          if (!ptx::mbar_wait(empty_bar(old_stage), old_phase)) {
+            mx_report_timeout(args.status, kStatusMmaTmemTimeout, cluster, static_cast<int>(i), abort_flag);
+            break;
+          }
+          if (++old_stage == args.stages) {
+            old_stage = 0;
+            old_phase ^= 1u;
+          }
         }
         if (!ptx::mbar_wait(full_bar(stage), phase)) {
-          mx_report_timeout(args.status, kStatusMmaFullTimeout, tile, kt, abort_flag);
-          ok = false;
+          mx_report_timeout(args.status, kStatusMmaFullTimeout, cluster, static_cast<int>(i), abort_flag);
           break;
         }
         ptx::tc_fence_after_sync();
-        const uint32_t x = stage_addr(stage), w = x + T::kXBytes, sx = w + T::kWBytes, sw = sx + T::kScaleTile;
-        const uint32_t tsx = tmem_base + T::kAccCols + (i % kMxScaleBuffers) * T::kScaleCols;
+        const uint32_t tsx = tmem_base + T::kScales0 + static_cast<uint32_t>(buffer * T::kScaleCols);
         const uint32_t tsw = tsx + T::kGroups * 4;
 #pragma unroll
         for (int g = 0; g < T::kGroups; ++g) {
-          ptx::tmem_copy_scales<1>(tsx + g * 4, make_smem_desc_scales(sx + g * kMxGroupBytes));
+          ptx::tmem_copy_scales<G>(tsx + g * 4, desc + g * (kMxGroupBytes >> 4));
 #pragma unroll
           for (int b = 0; b < T::kSBlocks; ++b) {
-            ptx::tmem_copy_scales<1>(tsw + (g * T::kSBlocks + b) * 4,
-                                     make_smem_desc_scales(sw + b * T::kScaleTile + g * kMxGroupBytes));
+            ptx::tmem_copy_scales<G>(tsw + (g * T::kSBlocks + b) * 4,
+                                     desc + ((b + 1) * T::kScaleTile + g * kMxGroupBytes) / 16);
           }
         }
-        const uint64_t dx = make_smem_desc_sw128(x), dw = make_smem_desc_sw128(w);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int g = FMT == kMxfp4 ? k / 2 : k;
-          ptx::umma_mxf4<1, FMT == kNvfp4>(tmem_base, dx + k * kDescKStep, dw + k * kDescKStep, (k & 1) ? idesc1 : idesc0,
-                                           tsx + g * 4, tsw + g * 4 * T::kSBlocks, (i > 0 || k > 0) ? 1u : 0u);
+        if (PAIR) {
+          ptx::umma_commit_pair(scales_bar(buffer), static_cast<uint16_t>(1u << leader));
+        } else {
+          ptx::umma_commit_1cta(scales_bar(buffer));
         }
-        ptx::umma_commit_1cta(empty_bar(stage));
+        desc += T::kStageBytes >> 4;
         if (++stage == args.stages) {
           stage = 0;
           phase ^= 1u;
+          desc = desc0;
         }
+        if (++buffer == T::kScaleBuffers) buffer = 0;
       }
-      if (ok) ptx::umma_commit_1cta(done_bar);
     }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;
+    const uint32_t slab0 = slab_base + static_cast<uint32_t>(q * args.slab_bytes);
+    const uint32_t leader_drained = PAIR ? ptx::map_to_cta(drained_bar(0), leader) : drained_bar(0);
+    constexpr int kChunk = BN < 32 ? BN : 32;
+    constexpr int kChunks = BN / kChunk;
+    constexpr int kFirst = T::kOverlap / 32;  // chunks that are handed back early
+    int turn = 0;
+    uint32_t stores = 0;
+    for (int tile = cluster; tile < args.sched.num_tiles; tile += args.sched.num_workers, ++turn) {
+      const TileCoord tc = tile_coord(args.sched, tile);
+      const int acc = turn & 1;
+      const int r_warp = tc.m * T::kTileRows + static_cast<int>(cta) * 128 + q * 32;  // this warp's first row
+      const int row = r_warp + static_cast<int>(lane);
+      const int s0 = tc.n * BN;
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(done_bar(acc), static_cast<uint32_t>(turn >> 1) & 1u))) {
+        if (lane == 0) mx_report_timeout(args.status, kStatusEpilogueTimeout, tile, acc, abort_flag);
+        break;
+      }
+      ptx::tc_fence_after_sync();
+      const uint32_t taddr = tmem_base + (acc ? T::kAcc1 : 0) + (static_cast<uint32_t>(q * 32) << 16);
+      auto hand_back = [&]() {
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          ptx::mbar_arrive_cluster(leader_drained + 8u * static_cast<uint32_t>(T::kOverlap > 0 ? 0 : acc));
+        }
+      };
+      if (args.split > 1) {
+        // Partial tile, column by column (the lanes of a warp write consecutive floats), over the ring:
+        // every load into it has been consumed. The cluster finishes it below.
+#pragma unroll 1
+        for (int c = 0; c < BN; c += kChunk) {
+          uint32_t v[kChunk];
+          ptx::tmem_ld_cols(taddr + c, v);
+          ptx::tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) {
+            ptx::st_shared_f32(smem_base + static_cast<uint32_t>(((c + j) * 128 + q * 32 + lane) * 4), __uint_as_float(v[j]));
+          }
+        }
+        break;
+      }
+      const bool live = r_warp < args.R;  // the same for the whole warp
+      // One 32-column piece of this lane's row, already in the output type, to C.
+      auto store = [&](const uint32_t (&p)[kChunk / 2], int c) {
+        if (!live || s0 + c >= args.S) return;
+        if (args.transposed) {
+          if (row < args.R) {
+#pragma unroll
+            for (int j = 0; j < kChunk; ++j) {
+              if (s0 + c + j < args.S) {
+                args.C[static_cast<long long>(s0 + c + j) * args.ldc + row] = static_cast<uint16_t>(p[j / 2] >> (16 * (j & 1)));
+              }
+            }
+          }
+          return;
+        }
+        if constexpr (BN >= 64) {
+          // 32 rows x 32 columns in a slab: as a 64-byte-swizzled box for a TMA store, or read back so that
+          // a warp writes runs of 32 elements of one row.
+          const uint32_t slab = slab0 + (stores & (kMxSlabs - 1)) * kMxSlabBytes;
+          ++stores;
+          if (args.tma_store && lane == 0) ptx::tma_store_wait_read<kMxSlabs - 1>();
+          __syncwarp();  // whoever used this slab last is done with it
+#pragma unroll
+          for (int j = 0; j < kChunk / 8; ++j) {
+            ptx::st_shared_v4(slab + lane * 64u + ((static_cast<uint32_t>(j) ^ ((lane >> 1) & 3u)) << 4), p[4 * j], p[4 * j + 1],
+                              p[4 * j + 2], p[4 * j + 3]);
+          }
+          if (args.tma_store) {
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              ptx::tma_store_3d(&map_c, slab, s0 + c, r_warp, 0);
+              ptx::tma_store_commit();
+            }
+          } else {
+            __syncwarp();
+            const bool column = s0 + c + static_cast<int>(lane) < args.S;
+            uint16_t* dst = args.C + static_cast<long long>(r_warp) * args.ldc + s0 + c + lane;
+#pragma unroll 8
+            for (int r = 0; r < 32; ++r) {
+              const uint32_t at = slab + r * 64u + (((lane >> 3) ^ ((static_cast<uint32_t>(r) >> 1) & 3u)) << 4) + (lane & 7u) * 2u;
+              const uint16_t h = ptx::ld_shared_u16(at);
+              if (column && r_warp + r < args.R) dst[static_cast<long long>(r) * args.ldc] = h;
+            }
+          }
+        }
+      };
+      auto pack = [&](const uint32_t (&v)[kChunk], uint32_t (&p)[kChunk / 2]) {
+#pragma unroll
+        for (int j = 0; j < kChunk / 2; ++j) {
+          p[j] = mx_pack16<F16>(mx_finish(args, __uint_as_float(v[2 * j])), mx_finish(args, __uint_as_float(v[2 * j + 1])));
+        }
+      };
+      int c_rest = 0;
+      if constexpr (kFirst > 0) {
+        // The overlapping chunks, the last ones of the first accumulator or the first of the second, are read out
+        // and handed back before anything is stored: the next tile waits for no more than this.
+        const int c_first = acc ? 0 : BN - T::kOverlap;
+        uint32_t p[kFirst][kChunk / 2];
+#pragma unroll
+        for (int i = 0; i < kFirst; ++i) {
+          uint32_t v[kChunk];
+          ptx::tmem_ld_cols(taddr + c_first + i * kChunk, v);
+          ptx::tmem_ld_wait();
+          pack(v, p[i]);
+        }
+        hand_back();
+#pragma unroll
+        for (int i = 0; i < kFirst; ++i) store(p[i], c_first + i * kChunk);
+        c_rest = acc ? T::kOverlap : 0;
+      }
+#pragma unroll 1
+      for (int i = 0; i < kChunks - kFirst; ++i) {
+        const int c = c_rest + i * kChunk;
+        uint32_t v[kChunk], p[kChunk / 2];
+        __syncwarp();
+        ptx::tmem_ld_cols(taddr + c, v);
+        ptx::tmem_ld_wait();
+        if (kFirst == 0 && i == kChunks - 1) hand_back();
+        pack(v, p);
+        store(p, c);
+      }
+    }
+    if (lane == 0) ptx::tma_store_wait<0>();
     __syncwarp();
   }
 
-  const int q = warp & 3;
-  const int row = q * 32 + static_cast<int>(lane);  // of the tile
-  bool ready = false;
-  if (warp >= 2) {
-    ready = __all_sync(0xffffffffu, ptx::mbar_wait(done_bar, 0));
-    if (!ready && lane == 0) mx_report_timeout(args.status, kStatusEpilogueTimeout, tile, 0, abort_flag);
-    ptx::tc_fence_after_sync();
-  }
-  const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
-  constexpr int kChunk = BN < 32 ? BN : 32;
-  if (split > 1) {
-    // Partial tile, column by column (the lanes of a warp write consecutive floats), over the ring:
-    // every load into it has been consumed.
-    if (warp >= 2 && ready) {
-#pragma unroll 1
-      for (int c = 0; c < BN; c += kChunk) {
-        uint32_t v[kChunk];
-        ptx::tmem_ld_cols(taddr + c, v);
-        ptx::tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          ptx::st_shared_f32(smem_base + static_cast<uint32_t>(((c + j) * 128 + row) * 4), __uint_as_float(v[j]));
-        }
-      }
-    }
+  if (args.split > 1) {
     __syncwarp();
     ptx::cluster_arrive();
     ptx::cluster_wait();
-    if (warp >= 2 && ready && r0 + row < args.R) {
-      // Rank r finishes columns [BN * r / split, BN * (r + 1) / split).
-      const int c0 = BN * rank / split, c1 = BN * (rank + 1) / split;
-      for (int c = c0; c < c1 && s0 + c < args.S; ++c) {
-        float sum = 0.0f;
-        for (int p = 0; p < split; ++p) {
-          sum += ptx::ld_cluster_f32(ptx::map_to_cta(smem_base + static_cast<uint32_t>((c * 128 + row) * 4), p));
-        }
-        const uint16_t h = static_cast<uint16_t>(mx_pack16<F16>(mx_finish(args, sum), 0.0f));
-        if (args.transposed) {
-          args.C[static_cast<long long>(s0 + c) * args.ldc + r0 + row] = h;
-        } else {
-          args.C[static_cast<long long>(r0 + row) * args.ldc + s0 + c] = h;
-        }
-      }
-    }
-    __syncwarp();
-    ptx::cluster_arrive();  // no CTA leaves while another still reads its partial tile
-    ptx::cluster_wait();
-  } else if (warp >= 2 && ready) {
-#pragma unroll 1
-    for (int c = 0; c < BN; c += kChunk) {
-      uint32_t v[kChunk];
-      __syncwarp();
-      ptx::tmem_ld_cols(taddr + c, v);
-      ptx::tmem_ld_wait();
-      if (r0 + row >= args.R) {
-        // a row of padding
-      } else if (args.transposed) {
+    if (*abort_flag == 0u) {
+      // Part p finishes columns [BN * p / split, BN * (p + 1) / split): a warp one column at a time, a lane
+      // four rows of it, four columns on the way (one at a time is a remote latency per column: 25 us for 128).
+      const TileCoord tc = tile_coord(args.sched, cluster);
+      const int s0 = tc.n * BN;
+      const int row = tc.m * T::kTileRows + static_cast<int>(cta) * 128 + static_cast<int>(lane) * 4;
+      const int c0 = BN * part / args.split;
+      const int c1 = min(BN * (part + 1) / args.split, args.S - s0);
+      const bool wide = row + 4 <= args.R && args.ldc % 4 == 0 && (reinterpret_cast<uintptr_t>(args.C) & 7u) == 0;
+      constexpr int kWarps = T::kThreads / 32, kAhead = 4;
+      for (int c = c0 + warp; c < c1 && row < args.R; c += kWarps * kAhead) {
+        float4 sum[kAhead];
 #pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          if (s0 + c + j < args.S) {
-            args.C[static_cast<long long>(s0 + c + j) * args.ldc + r0 + row] =
-                static_cast<uint16_t>(mx_pack16<F16>(mx_finish(args, __uint_as_float(v[j])), 0.0f));
+        for (int u = 0; u < kAhead; ++u) sum[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int p = 0; p < args.split; ++p) {
+          const uint32_t peer = ptx::map_to_cta(smem_base, p * G + cta);
+#pragma unroll
+          for (int u = 0; u < kAhead; ++u) {
+            if (c + u * kWarps < c1) {
+              const float4 v = ptx::ld_cluster_v4(peer + static_cast<uint32_t>(((c + u * kWarps) * 128 + lane * 4) * 4));
+              sum[u].x += v.x;
+              sum[u].y += v.y;
+              sum[u].z += v.z;
+              sum[u].w += v.w;
+            }
           }
         }
-      } else {
-        uint16_t* dst = args.C + static_cast<long long>(r0 + row) * args.ldc + s0 + c;
 #pragma unroll
-        for (int j = 0; j < kChunk; j += 8) {
-          uint32_t p[4];
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            p[h] = mx_pack16<F16>(mx_finish(args, __uint_as_float(v[j + 2 * h])),
-                                  mx_finish(args, __uint_as_float(v[j + 2 * h + 1])));
-          }
-          if (args.vec) {
-            if (s0 + c + j < args.S) *reinterpret_cast<uint4*>(dst + j) = make_uint4(p[0], p[1], p[2], p[3]);
+        for (int u = 0; u < kAhead; ++u) {
+          if (c + u * kWarps >= c1) break;
+          uint16_t* dst = args.C + static_cast<long long>(s0 + c + u * kWarps) * args.ldc + row;
+          const uint32_t lo = mx_pack16<F16>(mx_finish(args, sum[u].x), mx_finish(args, sum[u].y));
+          const uint32_t hi = mx_pack16<F16>(mx_finish(args, sum[u].z), mx_finish(args, sum[u].w));
+          if (wide) {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(lo, hi);
           } else {
 #pragma unroll
-            for (int h = 0; h < 8; ++h) {
-              if (s0 + c + j + h < args.S) dst[j + h] = static_cast<uint16_t>(p[h / 2] >> (16 * (h & 1)));
+            for (int h = 0; h < 4; ++h) {
+              if (row + h < args.R) dst[h] = static_cast<uint16_t>((h < 2 ? lo : hi) >> (16 * (h & 1)));
             }
           }
         }
       }
     }
+    __syncwarp();
   }
 
   ptx::tc_fence_before_sync();
@@ -318,9 +525,14 @@ __global__ void __launch_bounds__(192) mx_gemm_kernel(const __grid_constant__ CU
     // A wait gave up: let copies in flight land before shared and tensor memory are released.
     for (int i = 0; i < 1000; ++i) __nanosleep(1000);
   }
+  if (cluster_size > 1) {
+    // No CTA leaves while another reads its partial tile, its barriers or its tensor memory.
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+  }
   if (warp == 1) {
     ptx::tc_fence_after_sync();
-    ptx::tmem_dealloc<1>(tmem_base, T::kTmemCols);
+    ptx::tmem_dealloc<G>(tmem_base, T::kTmemCols);
   }
 }
 

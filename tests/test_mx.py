@@ -449,3 +449,26 @@ def test_streams_capture_and_repeat():
             graph.replay()
         assert all(torch.equal(result, expect) for _, result in graphs)
     assert g.device_status()[0] == api.STATUS_OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(65, 8200, 1100), (256, 18944, 512), (257, 19000, 300), (300, 256, 9000), (2100, 4800, 1030), (3000, 2999, 257),
+                                   (16, 40000, 300), (64, 38000, 700), (1, 60000, 256), (4097, 513, 2048), (600, 600, 24000)])
+def test_product_many_tiles(M, N, K, fmt):
+    """More tiles than the device takes at a time, ragged ends, long contractions shared by a cluster."""
+    low, high = (125, 129) if fmt == "mxfp4" else (0x28, 0x40)
+    a, av = random_mx(M, K, fmt, M + N, low, high)
+    b, bv = random_mx(N, K, fmt, K + 3, low, high)
+    out = torch.full((M, N), math.nan, dtype=torch.bfloat16, device="cuda")
+    g.gemm_mx(a, b, out=out)
+    bad = 0
+    bv32 = torch.from_numpy(bv).cuda()
+    for r in range(0, M, 512):  # (in slices: the reference is 64-bit)
+        rows = torch.from_numpy(av[r:r + 512]).cuda()
+        ref = rows @ bv32.T
+        bound = 2.0 ** -8 * ref.abs() + (K / 64 + 9) * 2.0 ** -22 * (rows.abs() @ bv32.abs().T)
+        bad += int((~((out[r:r + 512].double() - ref).abs() <= bound)).sum())
+    assert bad == 0, f"{bad} of {M * N} outside"
+    assert torch.equal(out, g.gemm_mx(a, b))
+    assert g.device_status()[0] == api.STATUS_OK
