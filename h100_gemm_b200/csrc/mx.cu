@@ -132,7 +132,15 @@ MxPlan plan_product(int M, int N, int K, int sms) {
   p.width = M <= 128 ? 128 : 256;
   const long long tiles = ceil_div(N, 256) * ceil_div(M, p.width);
   while (p.split < 4 && tiles * (p.split + 1) <= sms / 2 && k_tiles >= 4ll * (p.split + 1)) ++p.split;
-  if (p.split == 1 && M > 256) p.transposed = 0;
+  if (p.split == 1 && M > 256) {
+    p.transposed = 0;
+    // Lone CTAs of 128 x 256 take about 1.2 times as long for their share (they load all of B's tile themselves:
+    // 4096 x 8192 x 4096 NVFP4 69 against 58 us), but halve what a partly filled last wave wastes
+    // (777 x 5008 x 4104: 80 tiles are two waves of 74 pairs, 140 half tiles one wave of 148, 16.1 against 21.3 us).
+    const long long pair_waves = ceil_div(tiles, sms / 2);
+    const long long lone_waves = ceil_div(ceil_div(M, 128) * ceil_div(N, 256), sms);
+    if (lone_waves * 6 < pair_waves * 5) p.pair = 0;
+  }
   return p;
 }
 
@@ -141,7 +149,8 @@ int launch_gemm(const DeviceInfo& dev, const MxProduct& p, const MxPlan& plan, M
   using T = MxGemmTraits<FMT, BN, PAIR>;
   args.k_tiles = static_cast<int>(mx_col_tiles(p.K));
   args.split = plan.split;
-  args.slab_bytes = plan.transposed ? 0 : kMxSlabs * kMxSlabBytes;
+  args.tma_store = !plan.transposed && aligned16(args.C) && args.ldc % 8 == 0 ? 1 : 0;
+  args.slab_bytes = plan.transposed ? 0 : args.tma_store ? kMxSlabs * kMxSlabBytes : 32 * kMxRowPitch;
   args.sched.tiles_m = static_cast<int>(ceil_div(p.R, T::kTileRows));
   args.sched.tiles_n = static_cast<int>(ceil_div(p.S, BN));
   args.sched.batch = 1;
@@ -169,7 +178,6 @@ int launch_gemm(const DeviceInfo& dev, const MxProduct& p, const MxPlan& plan, M
   if (rc == B200_OK) rc = scale_map(dev, &msx, FMT, p.sx, p.R, p.K);
   if (rc == B200_OK) rc = scale_map(dev, &msw, FMT, p.sw, p.S, p.K);
   if (rc != B200_OK) return rc;
-  args.tma_store = !plan.transposed && aligned16(args.C) && args.ldc % 8 == 0 ? 1 : 0;
   if (args.tma_store) {
     rc = tile_map(dev, &mc, CU_TENSOR_MAP_DATA_TYPE_UINT16, args.C, static_cast<uint64_t>(p.S), static_cast<uint64_t>(p.R),
                   static_cast<uint64_t>(args.ldc) * 2, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B);
@@ -195,7 +203,9 @@ int launch_gemm(const DeviceInfo& dev, const MxProduct& p, const MxPlan& plan, c
     case 32: return launch_gemm<FMT, 32, 0, F16>(dev, p, plan, args, stream);
     case 64: return launch_gemm<FMT, 64, 0, F16>(dev, p, plan, args, stream);
     case 128: return launch_gemm<FMT, 128, 1, F16>(dev, p, plan, args, stream);
-    default: return launch_gemm<FMT, 256, 1, F16>(dev, p, plan, args, stream);
+    default:
+      return plan.pair ? launch_gemm<FMT, 256, 1, F16>(dev, p, plan, args, stream)
+                       : launch_gemm<FMT, 256, 0, F16>(dev, p, plan, args, stream);
   }
 }
 

@@ -56,6 +56,11 @@ struct MxGemmArgs {
 static constexpr int kMxMaxStages = 16;
 static constexpr int kMxSlabBytes = 32 * 64;  // 32 rows x 32 columns of 16-bit output
 static constexpr int kMxSlabs = 2;            // per epilogue warp
+// Rows of C that do not start on 16 bytes: a warp stages 32 rows of 128 columns (16 bytes of padding against bank
+// conflicts) and writes them as aligned 16-byte pieces; element by element, the partial sectors cost
+// 777 x 5003 x 4104 NVFP4 18 us of 36.
+static constexpr int kMxRowCols = 128;
+static constexpr int kMxRowPitch = 2 * kMxRowCols + 16;
 
 template <int FMT, int BN, int PAIR>
 struct MxGemmTraits {
@@ -70,9 +75,9 @@ struct MxGemmTraits {
   static constexpr int kGroups = mx_tile_groups(FMT);
   static constexpr int kStageBytes = kXBytes + kWBytes + (1 + kSBlocks) * kScaleTile;
   static constexpr int kScaleCols = kGroups * 4 * (1 + kSBlocks);   // of one K-tile: X's, then W's
-  // K-tiles whose scales tensor memory holds; never more than the ring has stages. NVFP4 has twice the scales: three
-  // where tensor memory (BN = 256) or half an SM's shared memory (BN = 64) has no room for a fourth.
-  static constexpr int kScaleBuffers = FMT == kNvfp4 && (BN == 256 || BN == 64) ? 3 : 4;
+  // K-tiles whose scales tensor memory holds; never more than the ring has stages. Three where tensor memory or the ring
+  // (BN = 256), or half an SM's shared memory (64, NVFP4) has no room for a fourth.
+  static constexpr int kScaleBuffers = BN == 256 || (FMT == kNvfp4 && BN == 64) ? 3 : 4;
   static constexpr int kScalesNeed = kScaleBuffers * kScaleCols;
   static constexpr int kAccCols = BN < 32 ? 32 : BN;
   // Columns the two accumulators share, in whole 32-column reads.
@@ -382,6 +387,41 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
         break;
       }
       const bool live = r_warp < args.R;  // the same for the whole warp
+      // The staged rows, columns [c, c + 128) of the tile: whole 16-byte pieces of C by 16 lanes per row, then what
+      // lies before and after them, a lane one row.
+      auto write_rows = [&](int c) {
+        __syncwarp();
+        const int cols = min(kMxRowCols, args.S - s0 - c);
+        auto at = [&](int r, uint16_t** dst) {
+          *dst = args.C + static_cast<long long>(r_warp + r) * args.ldc + s0 + c;
+          const int head = static_cast<int>((16u - (reinterpret_cast<uintptr_t>(*dst) & 15u)) & 15u) / 2;
+          return head < cols ? head : cols;
+        };
+#pragma unroll 4
+        for (int r = static_cast<int>(lane >> 4); r < 32; r += 2) {
+          uint16_t* dst;
+          const int e = at(r, &dst) + static_cast<int>(lane & 15u) * 8;
+          if (r_warp + r >= args.R || e + 8 > cols) continue;
+          const uint32_t src = slab0 + static_cast<uint32_t>(r * kMxRowPitch + (e >> 1) * 4);
+          uint32_t w[5];
+#pragma unroll
+          for (int k = 0; k < 5; ++k) w[k] = (k < 4 || (e & 1)) ? ptx::ld_shared_u32(src + k * 4) : 0u;
+          if (e & 1) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], 16);
+          }
+          *reinterpret_cast<uint4*>(dst + e) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (row < args.R) {
+          uint16_t* dst;
+          const int head = at(static_cast<int>(lane), &dst);
+          const int tail = head + (cols - head) / 8 * 8;
+          const uint32_t src = slab0 + lane * kMxRowPitch;
+          for (int k = 0; k < head; ++k) dst[k] = ptx::ld_shared_u16(src + static_cast<uint32_t>(k * 2));
+          for (int k = tail; k < cols; ++k) dst[k] = ptx::ld_shared_u16(src + static_cast<uint32_t>(k * 2));
+        }
+        __syncwarp();  // before the rows are overwritten
+      };
       // One 32-column piece of this lane's row, already in the output type, to C.
       auto store = [&](const uint32_t (&p)[kChunk / 2], int c) {
         if (!live || s0 + c >= args.S) return;
@@ -397,18 +437,17 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
           return;
         }
         if constexpr (BN >= 64) {
-          // 32 rows x 32 columns in a slab: as a 64-byte-swizzled box for a TMA store, or read back so that
-          // a warp writes runs of 32 elements of one row.
-          const uint32_t slab = slab0 + (stores & (kMxSlabs - 1)) * kMxSlabBytes;
-          ++stores;
-          if (args.tma_store && lane == 0) ptx::tma_store_wait_read<kMxSlabs - 1>();
-          __syncwarp();  // whoever used this slab last is done with it
-#pragma unroll
-          for (int j = 0; j < kChunk / 8; ++j) {
-            ptx::st_shared_v4(slab + lane * 64u + ((static_cast<uint32_t>(j) ^ ((lane >> 1) & 3u)) << 4), p[4 * j], p[4 * j + 1],
-                              p[4 * j + 2], p[4 * j + 3]);
-          }
           if (args.tma_store) {
+            // 32 rows x 32 columns as a 64-byte-swizzled box for a TMA store
+            const uint32_t slab = slab0 + (stores & (kMxSlabs - 1)) * kMxSlabBytes;
+            ++stores;
+            if (lane == 0) ptx::tma_store_wait_read<kMxSlabs - 1>();
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < kChunk / 8; ++j) {
+              ptx::st_shared_v4(slab + lane * 64u + ((static_cast<uint32_t>(j) ^ ((lane >> 1) & 3u)) << 4), p[4 * j], p[4 * j + 1],
+                                p[4 * j + 2], p[4 * j + 3]);
+            }
             ptx::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -416,15 +455,12 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
               ptx::tma_store_commit();
             }
           } else {
-            __syncwarp();
-            const bool column = s0 + c + static_cast<int>(lane) < args.S;
-            uint16_t* dst = args.C + static_cast<long long>(r_warp) * args.ldc + s0 + c + lane;
-#pragma unroll 8
-            for (int r = 0; r < 32; ++r) {
-              const uint32_t at = slab + r * 64u + (((lane >> 3) ^ ((static_cast<uint32_t>(r) >> 1) & 3u)) << 4) + (lane & 7u) * 2u;
-              const uint16_t h = ptx::ld_shared_u16(at);
-              if (column && r_warp + r < args.R) dst[static_cast<long long>(r) * args.ldc] = h;
+#pragma unroll
+            for (int j = 0; j < kChunk / 8; ++j) {
+              ptx::st_shared_v4(slab0 + lane * kMxRowPitch + static_cast<uint32_t>(c % kMxRowCols * 2 + j * 16), p[4 * j],
+                                p[4 * j + 1], p[4 * j + 2], p[4 * j + 3]);
             }
+            if ((c + kChunk) % kMxRowCols == 0 || s0 + c + kChunk >= args.S) write_rows(c / kMxRowCols * kMxRowCols);
           }
         }
       };
@@ -434,10 +470,21 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
           p[j] = mx_pack16<F16>(mx_finish(args, __uint_as_float(v[2 * j])), mx_finish(args, __uint_as_float(v[2 * j + 1])));
         }
       };
-      int c_rest = 0;
+      auto store_rest = [&](int c_begin, int c_end) {
+#pragma unroll 1
+        for (int c = c_begin; c < c_end; c += kChunk) {
+          uint32_t v[kChunk], p[kChunk / 2];
+          __syncwarp();
+          ptx::tmem_ld_cols(taddr + c, v);
+          ptx::tmem_ld_wait();
+          if (kFirst == 0 && c + kChunk == BN) hand_back();
+          pack(v, p);
+          store(p, c);
+        }
+      };
       if constexpr (kFirst > 0) {
         // The overlapping chunks, the last ones of the first accumulator or the first of the second, are read out
-        // and handed back before anything is stored: the next tile waits for no more than this.
+        // and handed back before anything is stored: the next tile waits for no more than this. Stores go from left to right.
         const int c_first = acc ? 0 : BN - T::kOverlap;
         uint32_t p[kFirst][kChunk / 2];
 #pragma unroll
@@ -448,20 +495,12 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
           pack(v, p[i]);
         }
         hand_back();
+        if (acc == 0) store_rest(0, c_first);
 #pragma unroll
         for (int i = 0; i < kFirst; ++i) store(p[i], c_first + i * kChunk);
-        c_rest = acc ? T::kOverlap : 0;
-      }
-#pragma unroll 1
-      for (int i = 0; i < kChunks - kFirst; ++i) {
-        const int c = c_rest + i * kChunk;
-        uint32_t v[kChunk], p[kChunk / 2];
-        __syncwarp();
-        ptx::tmem_ld_cols(taddr + c, v);
-        ptx::tmem_ld_wait();
-        if (kFirst == 0 && i == kChunks - 1) hand_back();
-        pack(v, p);
-        store(p, c);
+        if (acc == 1) store_rest(T::kOverlap, BN);
+      } else {
+        store_rest(0, BN);
       }
     }
     if (lane == 0) ptx::tma_store_wait<0>();

@@ -383,6 +383,11 @@ B200_DEVICE float4 ld_cluster_v4(uint32_t addr) {
   return v;
 }
 
+B200_DEVICE uint32_t ld_shared_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 B200_DEVICE uint16_t ld_shared_u16(uint32_t addr) {
   uint16_t v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");

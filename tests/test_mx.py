@@ -454,7 +454,7 @@ def test_streams_capture_and_repeat():
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("M,N,K", [(65, 8200, 1100), (256, 18944, 512), (257, 19000, 300), (300, 256, 9000), (2100, 4800, 1030), (3000, 2999, 257),
-                                   (16, 40000, 300), (64, 38000, 700), (1, 60000, 256), (4097, 513, 2048), (600, 600, 24000)])
+                                   (16, 40000, 300), (64, 38000, 700), (1, 60000, 256), (4097, 513, 2048), (600, 600, 24000), (777, 5008, 1100), (777, 5003, 1100), (900, 4610, 600), (300, 40001, 300)])
 def test_product_many_tiles(M, N, K, fmt):
     """More tiles than the device takes at a time, ragged ends, long contractions shared by a cluster."""
     low, high = (125, 129) if fmt == "mxfp4" else (0x28, 0x40)
