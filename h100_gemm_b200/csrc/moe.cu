@@ -24,9 +24,9 @@ bool sizes_ok(int T, int E, int k, int H, int I) {
 struct Launch {
   cudaLaunchConfig_t config = {};
   cudaLaunchAttribute attr[2];
-  Launch(int grid, int smem, cudaStream_t stream, int cluster) {
+  Launch(int grid, int threads, int smem, cudaStream_t stream, int cluster) {
     config.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-    config.blockDim = dim3(kMoeThreads, 1, 1);
+    config.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
     config.dynamicSmemBytes = static_cast<size_t>(smem);
     config.stream = stream;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -40,49 +40,39 @@ struct Launch {
   }
 };
 
-template <int W, int F16, int NT>
-int launch_down(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) {
-  constexpr int MT = MoeUnit<W>::kTiles;
-  const int units = (args.H + 16 * MT - 1) / (16 * MT);
-  const int smem = kMoeWarps * MT * NT * 32 * 16 + route_table_bytes(args.E, args.T * args.k);
-  // Clusters share a unit until every SM has two CTAs, but no warp is left without a step.
-  const int most = args.T * args.k < args.E ? args.T * args.k : args.E;
-  const long long steps = static_cast<long long>(most) * ((args.I + kMoeStep - 1) / kMoeStep);
-  int split = 1;
-  while (split < 8 && units * split * 2 <= dev.sm_count * 2 && steps >= 2ll * split * kMoeWarps) split *= 2;
-  const auto kernel = &moe_down_kernel<W, F16, NT>;
-  static std::atomic<bool> allowed[64];
-  const int rc = allow_shared_memory(dev, kernel, allowed);
-  if (rc != B200_OK) return rc;
-  Launch l(units * split, smem, stream, split);
-  B200_TRY_CUDA(cudaLaunchKernelEx(&l.config, kernel, args, split));
-  return B200_OK;
-}
-
 template <int W, int F16>
 int launch_all(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) {
-  const int clusters = (args.T + kRouterTokens - 1) / kRouterTokens;
-  Launch route(clusters * kRouterCluster, 0, stream, kRouterCluster);
-  B200_TRY_CUDA(cudaLaunchKernelEx(&route.config, &moe_router_kernel<F16>, args));
+  static std::atomic<bool> up_allowed[64], down_allowed[64];
+  int rc = allow_shared_memory(dev, &moe_gate_up_kernel<W, F16>, up_allowed);
+  if (rc == B200_OK) rc = allow_shared_memory(dev, &moe_down_kernel<W, F16>, down_allowed);
+  if (rc != B200_OK) return rc;
+
+  // One token alone has no company to share the router's rows with.
+  const int group = args.T == 1 ? 1 : kRouterTokens;
+  Launch route((args.T + group - 1) / group * kRouterCluster, kRouterThreads, 0, stream, kRouterCluster);
+  if (group == 1) {
+    B200_TRY_CUDA(cudaLaunchKernelEx(&route.config, &moe_router_kernel<F16, 1>, args));
+  } else {
+    B200_TRY_CUDA(cudaLaunchKernelEx(&route.config, &moe_router_kernel<F16, kRouterTokens>, args));
+  }
 
   constexpr int MT = MoeUnit<W>::kTiles;
-  const int most = args.T * args.k < args.E ? args.T * args.k : args.E;
+  const int tables = route_table_bytes(args.E, args.T * args.k);
+  const int most = args.T * args.k < args.E ? args.T * args.k : args.E;  // experts that can be chosen
   const long long units = static_cast<long long>(most) * ((args.I + 8 * MT - 1) / (8 * MT));
-  const int grid = static_cast<int>(units < 2ll * dev.sm_count ? units : 2ll * dev.sm_count);
-  const int smem = 2 * kMoeWarps * 32 * 16 * MT * moe_token_tiles(args.T) + route_table_bytes(args.E, args.T * args.k);
-  const auto kernel = &moe_gate_up_kernel<W, F16>;
-  static std::atomic<bool> allowed[64];
-  const int rc = allow_shared_memory(dev, kernel, allowed);
-  if (rc != B200_OK) return rc;
-  Launch up(grid, smem, stream, 1);
-  B200_TRY_CUDA(cudaLaunchKernelEx(&up.config, kernel, args));
+  Launch up(static_cast<int>(units < 2ll * dev.sm_count ? units : 2ll * dev.sm_count), kMoeThreads,
+            2 * kMoeWarps * gate_up_stride(MT, args.T) * 16 + tables, stream, 1);
+  B200_TRY_CUDA(cudaLaunchKernelEx(&up.config, &moe_gate_up_kernel<W, F16>, args));
 
-  switch (moe_token_tiles(args.T)) {
-    case 1: return launch_down<W, F16, 1>(dev, args, stream);
-    case 2: return launch_down<W, F16, 2>(dev, args, stream);
-    case 4: return launch_down<W, F16, 4>(dev, args, stream);
-    default: return launch_down<W, F16, 8>(dev, args, stream);
-  }
+  // Clusters share the columns of a unit until every SM has two CTAs, but no warp is left without a step.
+  const int columns = (args.H + 16 * MT - 1) / (16 * MT);
+  const long long steps = static_cast<long long>(most) * ((args.I + kMoeStep - 1) / kMoeStep);
+  int split = 1;
+  while (split < 8 && columns * split * 2 <= dev.sm_count * 2 && steps >= 2ll * split * kMoeWarps) split *= 2;
+  Launch down(columns * split, kMoeThreads, (kMoeWarps * args.T * Down<W, F16>::kPitch * 4 + 15) / 16 * 16 + tables, stream,
+              split);
+  B200_TRY_CUDA(cudaLaunchKernelEx(&down.config, &moe_down_kernel<W, F16>, args, split));
+  return B200_OK;
 }
 
 }  // namespace

@@ -22,6 +22,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "mx_format.cuh"
 #include "ptx.cuh"
 
@@ -34,7 +36,8 @@ static constexpr int kMoeThreads = 256;
 static constexpr int kMoeWarps = kMoeThreads / 32;
 static constexpr int kMoeStep = 256;         // elements of the contraction one warp takes at a time
 static constexpr int kRouterCluster = 8;
-static constexpr int kRouterTokens = 4;      // tokens one cluster routes
+static constexpr int kRouterThreads = 512;
+static constexpr int kRouterTokens = 4;      // tokens one cluster routes, at most
 
 enum MoeWeights : int { kMoe16 = 0, kMoeMxfp4 = 1, kMoeNvfp4 = 2 };
 
@@ -106,38 +109,52 @@ B200_DEVICE float key_logit(uint32_t key) {
 }
 static constexpr uint32_t kKeyMinusInf = 0x007FFFFFu;  // logit_key(-inf)
 
-// A cluster of 8 CTAs routes up to 4 tokens: CTA r has the experts [E r / 8, E (r + 1) / 8), a warp one expert
+// A cluster of 8 CTAs routes TOKENS tokens: CTA r has the experts [E r / 8, E (r + 1) / 8), a warp one expert
 // at a time against all tokens of the cluster; the logits of token j go to CTA j, whose first warp chooses.
-// Lanes hold the same elements of a dot product whatever T is, so a token's logits do not depend on its company.
-template <int F16>
-__global__ void __launch_bounds__(kMoeThreads) moe_router_kernel(const __grid_constant__ MoeArgs args) {
+// Bound by latency, so the loads of 1024 elements of every row are on the way together (with a branch
+// around each token's the kernel took 29 us for 4 tokens; now FIGURE_ROUTER). Lanes hold the same elements of a
+// dot product whatever T is, so a token's logits do not depend on its company.
+template <int F16, int TOKENS>
+__global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid_constant__ MoeArgs args) {
   __shared__ float logits[kMoeMaxExperts];
   const int warp = static_cast<int>(threadIdx.x) / 32;
   const int lane = static_cast<int>(threadIdx.x) % 32;
   const int rank = static_cast<int>(ptx::cluster_ctarank());
-  const int t0 = static_cast<int>(blockIdx.x) / kRouterCluster * kRouterTokens;
-  const int tokens = min(kRouterTokens, args.T - t0);
+  const int t0 = static_cast<int>(blockIdx.x) / kRouterCluster * TOKENS;
+  const int tokens = min(TOKENS, args.T - t0);
   ptx::grid_launch_dependents();
-  ptx::grid_dependency_wait();
   ptx::cluster_arrive();  // every CTA of the cluster runs before anyone writes into another's shared memory
   ptx::cluster_wait();
+  ptx::grid_dependency_wait();
   const int e_end = args.E * (rank + 1) / kRouterCluster;
   const uint32_t logits_addr = ptx::smem_u32(logits);
-  for (int e = args.E * rank / kRouterCluster + warp; e < e_end; e += kMoeWarps) {
-    float acc[kRouterTokens][2] = {};
+  const uint16_t* xrow[TOKENS];
+#pragma unroll
+  for (int j = 0; j < TOKENS; ++j) xrow[j] = args.x + static_cast<long long>(min(t0 + j, args.T - 1)) * args.H;
+  for (int e = args.E * rank / kRouterCluster + warp; e < e_end; e += kRouterThreads / 32) {
+    float acc[TOKENS][2] = {};
     const uint16_t* w = args.router + static_cast<long long>(e) * args.H;
-#pragma unroll 4
-    for (int c = lane * 8; c < args.H; c += 256) {
-      const uint4 q = *reinterpret_cast<const uint4*>(w + c);
-      const uint32_t qw[4] = {q.x, q.y, q.z, q.w};
+    for (int base = 0; base < args.H; base += 1024) {
+      uint4 q[4], v[TOKENS][4];
 #pragma unroll
-      for (int j = 0; j < kRouterTokens; ++j) {
-        if (j < tokens) {
-          const uint4 v = *reinterpret_cast<const uint4*>(args.x + static_cast<long long>(t0 + j) * args.H + c);
-          const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+      for (int i = 0; i < 4; ++i) {
+        // (beyond the row: its last elements again, not used)
+        const int c = base + i * 256 + lane * 8;
+        const int at = min(c, args.H - 8);
+        q[i] = *reinterpret_cast<const uint4*>(w + at);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 a = unpack16<F16>(qw[i]), b = unpack16<F16>(vw[i]);
+        for (int j = 0; j < TOKENS; ++j) v[j][i] = *reinterpret_cast<const uint4*>(xrow[j] + at);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (base + i * 256 + lane * 8 >= args.H) continue;
+        const uint32_t qw[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+        for (int j = 0; j < TOKENS; ++j) {
+          const uint32_t vw[4] = {v[j][i].x, v[j][i].y, v[j][i].z, v[j][i].w};
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const float2 a = unpack16<F16>(qw[h]), b = unpack16<F16>(vw[h]);
             acc[j][0] = fmaf(a.x, b.x, acc[j][0]);
             acc[j][1] = fmaf(a.y, b.y, acc[j][1]);
           }
@@ -146,7 +163,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_router_kernel(const __grid_co
     }
     const float bias = args.bias != nullptr ? args.bias[e] : 0.0f;
 #pragma unroll
-    for (int j = 0; j < kRouterTokens; ++j) {
+    for (int j = 0; j < TOKENS; ++j) {
       float s = acc[j][0] + acc[j][1];
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
@@ -221,23 +238,26 @@ __global__ void __launch_bounds__(kMoeThreads) moe_router_kernel(const __grid_co
 // expert and token.
 struct RouteTables {
   unsigned long long* mask;  // [E]
+  float* weights;            // routing weight of a pair
+  uint16_t* pairs;           // [T * k] token * k + choice
   uint16_t* list;            // [E] chosen experts, ascending
   uint16_t* first;           // [E] first pair of an expert in `pairs`
-  uint16_t* pairs;           // [T * k] token * k + choice
+  uint8_t* tokens;           // token of a pair
   int* count;                // chosen experts
 };
 
-__host__ __device__ __forceinline__ int route_table_bytes(int E, int pairs) {
-  return E * 8 + E * 2 + E * 2 + pairs * 2 + 16 + 16;
-}
+__host__ __device__ __forceinline__ int route_table_bytes(int E, int pairs) { return (E * 12 + pairs * 7 + 16 + 15) / 16 * 16; }
 
 B200_DEVICE RouteTables route_tables_at(uint8_t* smem, const MoeArgs& args) {
+  const int pairs = args.T * args.k;
   RouteTables r;
   r.mask = reinterpret_cast<unsigned long long*>(smem);
-  r.count = reinterpret_cast<int*>(smem + args.E * 8);
-  r.list = reinterpret_cast<uint16_t*>(smem + args.E * 8 + 16);
+  r.weights = reinterpret_cast<float*>(r.mask + args.E);
+  r.count = reinterpret_cast<int*>(r.weights + pairs);
+  r.pairs = reinterpret_cast<uint16_t*>(r.count + 1);
+  r.list = r.pairs + pairs;
   r.first = r.list + args.E;
-  r.pairs = r.first + args.E;
+  r.tokens = reinterpret_cast<uint8_t*>(r.first + args.E);
   return r;
 }
 
@@ -274,8 +294,11 @@ B200_DEVICE void build_route_tables(const RouteTables& r, const MoeArgs& args) {
   for (int p = t; p < pairs; p += kMoeThreads) {
     const int e = __ldcg(args.ids + p);
     if (e >= 0) {
-      const unsigned long long lower = r.mask[e] & ((1ull << (p / args.k)) - 1ull);
-      r.pairs[r.first[e] + __popcll(lower)] = static_cast<uint16_t>(p);
+      const int token = p / args.k;
+      const int at = r.first[e] + __popcll(r.mask[e] & ((1ull << token) - 1ull));
+      r.pairs[at] = static_cast<uint16_t>(p);
+      r.tokens[at] = static_cast<uint8_t>(token);
+      r.weights[at] = __ldcg(args.weights + p);
     }
   }
   __syncthreads();
@@ -283,61 +306,84 @@ B200_DEVICE void build_route_tables(const RouteTables& r, const MoeArgs& args) {
 
 // ------------------------------------------------------------------------------------- weights in registers
 // One warp's share of a step: MT x 16 weight rows against kMoeStep elements from k0 on. Row g of MMA m
-// is `rows(m, 0)`, row g + 8 is `rows(m, 1)` (negative: zeros). B operands come from `cols(j, &any)`, the vector
-// of column g of n-tile j (NULL: zeros; any = false: no column of the tile is in use).
+// is `rows(m, 0)`, row g + 8 is `rows(m, 1)` (negative: zeros). load() only issues the loads; mma() multiplies with
+// one n-tile, whose column g is the vector `b`.
 //
 // 16-bit weights: eight chunks of 32 elements, a lane 16 bytes of each row and chunk.
-template <int F16, int NT, int MT, typename Rows, typename Cols>
-B200_DEVICE void weight_step16(float (&acc)[MT][NT][4], const MoeMatrix& w, int k0, int K, uint32_t lane, Rows rows,
-                               Cols cols) {
-  const int kl = k0 + static_cast<int>(lane & 3u) * 8;
+template <int W, int F16, int MT>
+struct WeightStep {
   uint4 q[MT][2][8];
+
+  template <typename Rows>
+  B200_DEVICE void load(const MoeMatrix& w, int k0, int K, uint32_t lane, Rows rows) {
+    const int kl = k0 + static_cast<int>(lane & 3u) * 8;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+    for (int m = 0; m < MT; ++m) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const long long row = rows(m, half);
-      const uint8_t* p = w.data + row * w.pitch + kl * 2;
+      for (int half = 0; half < 2; ++half) {
+        const long long row = rows(m, half);
+        const uint8_t* p = w.data + row * w.pitch + kl * 2;
+        if (row >= 0 && k0 + kMoeStep <= K) {
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        q[m][half][c] = (row >= 0 && kl + c * 32 < K) ? ptx::ld_stream_v4(p + c * 64) : make_uint4(0u, 0u, 0u, 0u);
+          for (int c = 0; c < 8; ++c) q[m][half][c] = ptx::ld_stream_v4(p + c * 64);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            q[m][half][c] = make_uint4(0u, 0u, 0u, 0u);
+            if (row >= 0 && kl + c * 32 < K) q[m][half][c] = ptx::ld_stream_v4(p + c * 64);
+          }
+        }
       }
     }
   }
+
+  B200_DEVICE void mma(float (&acc)[MT][4], const uint16_t* b, int k0, int K, uint32_t lane) const {
+    const int kl = k0 + static_cast<int>(lane & 3u) * 8;
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    bool any;
-    const uint16_t* b = cols(j, &any);
-    if (!any) continue;  // (the same for the whole warp)
+    for (int c0 = 0; c0 < 8; c0 += 4) {  // (all eight at once would spill)
+      uint4 v[4];
+      if (k0 + kMoeStep <= K) {
 #pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      const uint4 v = (b != nullptr && kl + c * 32 < K) ? *reinterpret_cast<const uint4*>(b + kl + c * 32)
-                                                        : make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < 4; ++c) v[c] = *reinterpret_cast<const uint4*>(b + kl + (c0 + c) * 32);
+      } else {
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        mma16816<F16>(acc[m][j], q[m][0][c].x, q[m][1][c].x, q[m][0][c].y, q[m][1][c].y, v.x, v.y);
-        mma16816<F16>(acc[m][j], q[m][0][c].z, q[m][1][c].z, q[m][0][c].w, q[m][1][c].w, v.z, v.w);
+        for (int c = 0; c < 4; ++c) {
+          v[c] = make_uint4(0u, 0u, 0u, 0u);
+          if (kl + (c0 + c) * 32 < K) v[c] = *reinterpret_cast<const uint4*>(b + kl + (c0 + c) * 32);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const uint4 &lo = q[m][0][c0 + c], &hi = q[m][1][c0 + c];
+          mma16816<F16>(acc[m], lo.x, hi.x, lo.y, hi.y, v[c].x, v[c].y);
+          mma16816<F16>(acc[m], lo.z, hi.z, lo.w, hi.w, v[c].z, v[c].w);
+        }
       }
     }
   }
-}
+};
 
 // What a 4-bit weight's bits are multiplied with. A code's magnitude bits at the top of a bf16 number's mantissa
-// and the bottom of its exponent read code * 2^-126; two factors (the second nearly always 1) bring them to
-// code * scale (MXFP4) or code * scale * 2^-16 (NVFP4, whose block scales reach 448: the rest is
-// applied to the sums). Every product is exact in bf16.
+// and the bottom of its exponent read code * 2^-126; the factor brings them to code * scale (MXFP4) or
+// code * scale * 2^-16 (NVFP4, whose block scales reach 448: the rest is applied to the sums). MXFP4
+// scales above 2 (byte > 128) need a second factor, 2^(byte - 128); a step without any skips it. Every product is
+// exact in bf16.
 static constexpr float kNvfp4Lift = 65536.0f;
 template <int W>
-B200_DEVICE void weight_factors(uint32_t byte, uint32_t* first, uint32_t* second) {
-  uint32_t f, s = 0x3F80u;
+B200_DEVICE uint32_t weight_factor(uint32_t byte) {
+  uint32_t f;
   if constexpr (W == kMoeMxfp4) {
     f = byte == 255u ? 0x7FC0u : min(byte + 126u, 254u) << 7;
-    if (byte > 128u) s = (byte - 1u) << 7;  // 2^(byte - 128)
   } else {
     f = __float_as_uint(e4m3_value(byte) * 1.298074214633707e33f) >> 16;  // 2^110
   }
-  *first = f | (f << 16);
-  *second = s | (s << 16);
+  return f | (f << 16);
+}
+B200_DEVICE uint32_t weight_second_factor(uint32_t byte) {
+  const uint32_t s = byte > 128u ? (byte - 1u) << 7 : 0x3F80u;
+  return s | (s << 16);
 }
 
 B200_DEVICE uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
@@ -349,87 +395,108 @@ B200_DEVICE uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 // 4-bit weights: two chunks of 128 elements, a lane 16 bytes = 32 elements of each row and chunk. Of a word's
 // eight codes, i and i + 4 are 16 bits apart: one shift brings both to their place in a bf16 pair, and B
 // takes its elements in the same order.
-template <int W, int NT, int MT, typename Rows, typename Cols>
-B200_DEVICE void weight_step4(float (&acc)[MT][NT][4], const MoeMatrix& w, int k0, int K, uint32_t lane, Rows rows,
-                              Cols cols) {
-  constexpr int FMT = W == kMoeMxfp4 ? kMxfp4 : kNvfp4;
-  constexpr int kBlocks = 32 / mx_block(FMT);  // block scales of a lane's 32 elements
-  const int part = static_cast<int>(lane & 3u);
+template <int W, int MT>
+struct WeightStep4 {
+  static constexpr int FMT = W == kMoeMxfp4 ? kMxfp4 : kNvfp4;
+  static constexpr int kBlocks = 32 / mx_block(FMT);  // block scales of a lane's 32 elements
   uint4 q[MT][2][2];
   uint32_t sb[MT][2][2];
+  bool wide;  // a scale needs its second factor
+
+  template <typename Rows>
+  B200_DEVICE void load(const MoeMatrix& w, int k0, int K, uint32_t lane, Rows rows) {
+    const int part = static_cast<int>(lane & 3u);
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+    for (int m = 0; m < MT; ++m) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const long long row = rows(m, half);
-      const uint8_t* p = w.data + row * w.pitch + k0 / 2 + part * 16;
-      const uint8_t* sp = w.scales + mx_scale_offset(FMT, row, k0 / mx_block(FMT) + part * kBlocks, w.col_tiles);
+      for (int half = 0; half < 2; ++half) {
+        const long long row = rows(m, half);
+        const uint8_t* p = w.data + row * w.pitch + k0 / 2 + part * 16;
+        const uint8_t* sp = w.scales + mx_scale_offset(FMT, row, k0 / mx_block(FMT) + part * kBlocks, w.col_tiles);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const bool live = row >= 0 && k0 + c * 128 + part * 32 < K;
-        q[m][half][c] = live ? ptx::ld_stream_v4(p + c * 64) : make_uint4(0u, 0u, 0u, 0u);
-        sb[m][half][c] = 0u;
-        if (live) {
-          if constexpr (FMT == kMxfp4) {
-            sb[m][half][c] = sp[c * kMxGroupBytes];
-          } else {
-            sb[m][half][c] = *reinterpret_cast<const uint16_t*>(sp + c * 2 * kMxGroupBytes);
+        for (int c = 0; c < 2; ++c) {
+          q[m][half][c] = make_uint4(0u, 0u, 0u, 0u);
+          sb[m][half][c] = 0u;
+          if (row >= 0 && k0 + c * 128 + part * 32 < K) {
+            q[m][half][c] = ptx::ld_stream_v4(p + c * 64);
+            if constexpr (FMT == kMxfp4) {
+              sb[m][half][c] = sp[c * kMxGroupBytes];
+            } else {
+              sb[m][half][c] = *reinterpret_cast<const uint16_t*>(sp + c * 2 * kMxGroupBytes);
+            }
           }
         }
       }
     }
   }
+
+  // Codes of word `word` of chunk `c` of one row, as four bf16 pairs.
+  template <bool WIDE>
+  B200_DEVICE void weights(uint32_t (&a)[4], int m, int half, int c, int word) const {
+    const uint4& v = q[m][half][c];
+    const uint32_t codes = word == 0 ? v.x : word == 1 ? v.y : word == 2 ? v.z : v.w;
+    const uint32_t byte = (sb[m][half][c] >> (kBlocks == 2 ? (word / 2) * 8 : 0)) & 0xFFu;
+    const uint32_t f = weight_factor<W>(byte);
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t mag = (i < 2 ? codes << (6 - 4 * i) : codes >> (4 * i - 6)) & 0x01C001C0u;
+      a[i] = mul_bf16x2(mag | ((codes << (12 - 4 * i)) & 0x80008000u), f);
+      if constexpr (WIDE) a[i] = mul_bf16x2(a[i], weight_second_factor(byte));
+    }
+  }
+
+  // NT n-tiles at once, so that a weight is unpacked once: column g of tile j is the vector b[j].
+  template <int NT, bool WIDE>
+  B200_DEVICE void mma(float (&acc)[NT][MT][4], const uint16_t* const (&b)[NT], int k0, int K, uint32_t lane) const {
+    const int part = static_cast<int>(lane & 3u);
 #pragma unroll
-    for (int word = 0; word < 4; ++word) {
-      const int k = k0 + c * 128 + part * 32 + word * 8;
-      uint32_t a[MT][2][4];
+    for (int c = 0; c < 2; ++c) {
+      const int kc = k0 + c * 128 + part * 32;
+      const bool live = kc + 32 <= K;
+      uint4 v0[4];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint4& v = q[m][half][c];
-          const uint32_t codes = word == 0 ? v.x : word == 1 ? v.y : word == 2 ? v.z : v.w;
-          uint32_t f, s;
-          weight_factors<W>((sb[m][half][c] >> (kBlocks == 2 ? (word / 2) * 8 : 0)) & 0xFFu, &f, &s);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t mag = (i < 2 ? codes << (6 - 4 * i) : codes >> (4 * i - 6)) & 0x01C001C0u;
-            const uint32_t bits = mag | ((codes << (12 - 4 * i)) & 0x80008000u);
-            uint32_t d = mul_bf16x2(bits, f);
-            if constexpr (W == kMoeMxfp4) d = mul_bf16x2(d, s);
-            a[m][half][i] = d;
-          }
-        }
+      for (int word = 0; word < 4; ++word) {
+        v0[word] = make_uint4(0u, 0u, 0u, 0u);
+        if (live || kc + word * 8 < K) v0[word] = *reinterpret_cast<const uint4*>(b[0] + kc + word * 8);
       }
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        bool any;
-        const uint16_t* b = cols(j, &any);
-        if (!any) continue;
-        const uint4 v = (b != nullptr && k < K) ? *reinterpret_cast<const uint4*>(b + k) : make_uint4(0u, 0u, 0u, 0u);
-        const uint32_t b0 = __byte_perm(v.x, v.z, 0x5410), b1 = __byte_perm(v.x, v.z, 0x7632);
-        const uint32_t b2 = __byte_perm(v.y, v.w, 0x5410), b3 = __byte_perm(v.y, v.w, 0x7632);
+      for (int word = 0; word < 4; ++word) {
+        uint32_t a[MT][2][4];
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          mma16816<0>(acc[m][j], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], b0, b1);
-          mma16816<0>(acc[m][j], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], b2, b3);
+          weights<WIDE>(a[m][0], m, 0, c, word);
+          weights<WIDE>(a[m][1], m, 1, c, word);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint4 v = v0[word];
+          if (j > 0) {
+            v = make_uint4(0u, 0u, 0u, 0u);
+            if (kc + word * 8 < K) v = *reinterpret_cast<const uint4*>(b[j] + kc + word * 8);
+          }
+          const uint32_t b0 = __byte_perm(v.x, v.z, 0x5410), b1 = __byte_perm(v.x, v.z, 0x7632);
+          const uint32_t b2 = __byte_perm(v.y, v.w, 0x5410), b3 = __byte_perm(v.y, v.w, 0x7632);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            mma16816<0>(acc[j][m], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], b0, b1);
+            mma16816<0>(acc[j][m], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], b2, b3);
+          }
         }
       }
     }
   }
-}
 
-template <int W, int F16, int NT, int MT, typename Rows, typename Cols>
-B200_DEVICE void weight_step(float (&acc)[MT][NT][4], const MoeMatrix& w, int k0, int K, uint32_t lane, Rows rows,
-                             Cols cols) {
-  if constexpr (W == kMoe16) {
-    weight_step16<F16, NT, MT>(acc, w, k0, K, lane, rows, cols);
-  } else {
-    weight_step4<W, NT, MT>(acc, w, k0, K, lane, rows, cols);
+  B200_DEVICE bool needs_second_factor() const {
+    if constexpr (W != kMoeMxfp4) return false;
+    uint32_t most = 0u;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = max(most, sb[m][i / 2][i % 2]);
+    }
+    return __any_sync(0xFFFFFFFFu, most > 128u);
   }
-}
+};
 
 // MMA tiles of weight rows a unit has: 4-bit rows are a quarter as long, so a unit takes two to keep as much on the way.
 template <int W>
@@ -438,177 +505,257 @@ struct MoeUnit {
   static constexpr float kLift = W == kMoeNvfp4 ? kNvfp4Lift : 1.0f;
 };
 
+// One step of either kind against NT tiles; `b[j]` is column g of tile j.
+template <int W, int F16, int NT>
+struct MoeStep {
+  static constexpr int MT = MoeUnit<W>::kTiles;
+  using Weights = typename std::conditional<W == kMoe16, WeightStep<W, F16, MT>, WeightStep4<W, MT>>::type;
+  static B200_DEVICE void mma(const Weights& w, float (&acc)[NT][MT][4], const uint16_t* const (&b)[NT], int k0, int K,
+                              uint32_t lane) {
+    if constexpr (W == kMoe16) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) w.mma(acc[j], b[j], k0, K, lane);
+    } else if (w.needs_second_factor()) {
+      w.template mma<NT, true>(acc, b, k0, K, lane);
+    } else {
+      w.template mma<NT, false>(acc, b, k0, K, lane);
+    }
+  }
+};
+
 B200_DEVICE float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
+
+// The tokens of an expert ride on the MMA's N in the order of its pairs, two n-tiles at a time (more would
+// need more registers than the weights leave). Columns beyond the last token repeat it and are not used.
 
 // ------------------------------------------------------------------------------------- gate and up
 // Unit: 8 intermediate columns per MMA tile of one chosen expert = 8 gate rows and the 8 up rows beside them, so that
-// a lane ends up with a gate value and its up value. The CTAs take units in turn.
-template <int W, int F16, int NT>
-B200_DEVICE void gate_up_unit(const MoeArgs& args, const RouteTables& r, float4* red, int e, int i0, int tokens) {
-  constexpr int MT = MoeUnit<W>::kTiles;
-  const uint32_t lane = ptx::lane_id();
-  const int warp = static_cast<int>(threadIdx.x) / 32;
-  const int g = static_cast<int>(lane >> 2);
-  const uint16_t* pairs = r.pairs + r.first[e];
-  const uint16_t* xrow[NT];
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    xrow[j] = j * 8 + g < tokens ? args.x + static_cast<long long>(pairs[j * 8 + g] / args.k) * args.H : nullptr;
+// a lane ends up with a gate value and its up value. The CTAs take units in turn; a warp issues the next
+// step's loads, of the next unit if need be, as soon as its MMAs have taken the registers, so that memory is busy
+// while the sums are joined.
+template <int W, int F16>
+struct GateUp {
+  static constexpr int MT = MoeUnit<W>::kTiles;
+  static constexpr int kCols = 8 * MT;
+  using Weights = typename MoeStep<W, F16, 1>::Weights;
+  const MoeArgs& args;
+  const RouteTables& r;
+  uint32_t lane;
+  int warp, strips, units;
+  Weights w;
+
+  B200_DEVICE void load(int unit, int k0) {
+    const int e = r.list[unit / strips];
+    const int i0 = unit % strips * kCols;
+    const long long row = static_cast<long long>(e) * 2 * args.I + i0 + (lane >> 2);
+    const int I = args.I;
+    w.load(args.w1, k0, args.H, lane,
+           [=](int m, int half) { return i0 + m * 8 < I ? row + m * 8 + (half ? I : 0) : -1ll; });
   }
-  const long long row0 = static_cast<long long>(e) * 2 * args.I + i0 + g;
-  float acc[MT][NT][4] = {};
-  for (int k0 = warp * kMoeStep; k0 < args.H; k0 += kMoeWarps * kMoeStep) {
-    weight_step<W, F16, NT, MT>(
-        acc, args.w1, k0, args.H, lane,
-        [&](int m, int half) { return i0 + m * 8 < args.I ? row0 + m * 8 + (half ? args.I : 0) : -1ll; },
-        [&](int j, bool* any) {
-          *any = j * 8 < tokens;
-          return xrow[j];
-        });
-  }
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
+
+  // The loaded step against tiles [j0, j0 + NT) of the unit's tokens; sums go to (first) or on top of `mine`.
+  template <int NT>
+  B200_DEVICE void tiles(float4* mine, int first_pair, int tokens, int j0, int k0, bool first) {
+    const uint16_t* b[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      red[((warp * MT + m) * NT + j) * 32 + lane] = make_float4(acc[m][j][0], acc[m][j][1], acc[m][j][2], acc[m][j][3]);
+      const int c = min((j0 + j) * 8 + static_cast<int>(lane >> 2), tokens - 1);
+      b[j] = args.x + static_cast<long long>(r.tokens[first_pair + c]) * args.H;
     }
-  }
-  __syncthreads();
-  for (int idx = static_cast<int>(threadIdx.x); idx < MT * NT * 32; idx += kMoeThreads) {
-    float4 s = red[idx];
+    float acc[NT][MT][4] = {};
+    MoeStep<W, F16, NT>::mma(w, acc, b, k0, args.H, lane);
 #pragma unroll
-    for (int p = 1; p < kMoeWarps; ++p) {
-      const float4 v = red[p * MT * NT * 32 + idx];
-      s.x += v.x;
-      s.y += v.y;
-      s.z += v.z;
-      s.w += v.w;
-    }
-    const int tile = idx / 32;
-    const int row = i0 + tile / NT * 8 + (idx % 32) / 4;
-    const int c = tile % NT * 8 + (idx % 4) * 2;
-    const float gate[2] = {s.x, s.y}, up[2] = {s.z, s.w};
-    if (row >= args.I) continue;
+    for (int j = 0; j < NT; ++j) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      if (c + n < tokens) {
-        const int pair = pairs[c + n];
-        const float p = __ldcg(args.weights + pair);
-        args.h[static_cast<long long>(pair) * args.I + row] = round16<F16>(p * (silu(gate[n] * args.lift1) * (up[n] * args.lift1)));
+      for (int m = 0; m < MT; ++m) {
+        float4* to = mine + ((j0 + j) * MT + m) * 32 + lane;
+        float4 v = make_float4(acc[j][m][0], acc[j][m][1], acc[j][m][2], acc[j][m][3]);
+        if (!first) {
+          const float4 o = *to;
+          v.x += o.x;
+          v.y += o.y;
+          v.z += o.z;
+          v.w += o.w;
+        }
+        *to = v;
       }
     }
   }
-}
 
-__host__ __device__ __forceinline__ int moe_token_tiles(int T) { return T <= 8 ? 1 : T <= 16 ? 2 : T <= 32 ? 4 : 8; }
+  // `red`: every warp's sums, `stride` float4 apart.
+  B200_DEVICE void run(float4* red, int stride, int unit, int e, int tokens) {
+    const int first_pair = r.first[e];
+    const int n_tiles = (tokens + 7) / 8;
+    float4* mine = red + warp * stride;
+    for (int k0 = warp * kMoeStep; k0 - warp * kMoeStep < args.H; k0 += kMoeWarps * kMoeStep) {
+      const bool first = k0 == warp * kMoeStep;
+      if (k0 < args.H) {
+        int j = 0;
+        for (; j + 1 < n_tiles; j += 2) tiles<2>(mine, first_pair, tokens, j, k0, first);
+        if (j < n_tiles) tiles<1>(mine, first_pair, tokens, j, k0, first);
+      } else if (first) {
+        for (int i = 0; i < n_tiles * MT; ++i) mine[i * 32 + lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+      const int k_next = k0 + kMoeWarps * kMoeStep;
+      if (k_next - warp * kMoeStep < args.H) {
+        if (k_next < args.H) load(unit, k_next);
+      } else if (unit + static_cast<int>(gridDim.x) < units && warp * kMoeStep < args.H) {
+        load(unit + static_cast<int>(gridDim.x), warp * kMoeStep);
+      }
+    }
+    __syncthreads();
+    // Four threads per hidden value, two warps' sums each.
+    const int i0 = unit % strips * kCols;
+    const int quarter = static_cast<int>(threadIdx.x) & 3;
+    for (int o = static_cast<int>(threadIdx.x) / 4; o < n_tiles * MT * 64; o += kMoeThreads / 4) {
+      const int tile = o / 64, row_in = o % 64 / 8, col = o % 8;
+      const float* at = reinterpret_cast<const float*>(red + 2 * quarter * stride + tile * 32 + row_in * 4 + col / 2) + (col & 1);
+      float gate = at[0] + at[stride * 4], up = at[2] + at[stride * 4 + 2];
+      gate += __shfl_xor_sync(0xFFFFFFFFu, gate, 1);
+      up += __shfl_xor_sync(0xFFFFFFFFu, up, 1);
+      gate += __shfl_xor_sync(0xFFFFFFFFu, gate, 2);
+      up += __shfl_xor_sync(0xFFFFFFFFu, up, 2);
+      const int c = tile / MT * 8 + col, row = i0 + tile % MT * 8 + row_in;
+      if (quarter == 0 && c < tokens && row < args.I) {
+        args.h[static_cast<long long>(r.pairs[first_pair + c]) * args.I + row] =
+            round16<F16>(r.weights[first_pair + c] * (silu(gate * args.lift1) * (up * args.lift1)));
+      }
+    }
+  }
+};
+
+__host__ __device__ __forceinline__ int moe_token_tiles(int T) { return (T + 7) / 8; }
+// float4 between two warps' sums: the padding keeps the four threads of a value on different banks.
+__host__ __device__ __forceinline__ int gate_up_stride(int tiles, int T) { return tiles * moe_token_tiles(T) * 32 + 2; }
 
 template <int W, int F16>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __grid_constant__ MoeArgs args) {
-  constexpr int kCols = 8 * MoeUnit<W>::kTiles;
+  constexpr int kCols = GateUp<W, F16>::kCols;
   extern __shared__ __align__(16) uint8_t smem[];
   float4* red = reinterpret_cast<float4*>(smem);  // two buffers, used in turn
-  const int red_bytes = kMoeWarps * 32 * 16 * MoeUnit<W>::kTiles * moe_token_tiles(args.T);
-  const RouteTables r = route_tables_at(smem + 2 * red_bytes, args);
+  const int stride = gate_up_stride(MoeUnit<W>::kTiles, args.T);
+  const RouteTables r = route_tables_at(smem + 2 * kMoeWarps * stride * 16, args);
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
   build_route_tables(r, args);
-  const int strips = (args.I + kCols - 1) / kCols;
-  const int units = *r.count * strips;
-  int turn = 0;
-  for (int u = static_cast<int>(blockIdx.x); u < units; u += static_cast<int>(gridDim.x), turn ^= 1) {
-    const int e = r.list[u / strips];
-    const int i0 = u % strips * kCols;
-    const int tokens = __popcll(r.mask[e]);
-    float4* buffer = red + turn * (red_bytes / 16);
-    if (tokens <= 8) {
-      gate_up_unit<W, F16, 1>(args, r, buffer, e, i0, tokens);
-    } else if (tokens <= 16) {
-      gate_up_unit<W, F16, 2>(args, r, buffer, e, i0, tokens);
-    } else if (tokens <= 32) {
-      gate_up_unit<W, F16, 4>(args, r, buffer, e, i0, tokens);
-    } else {
-      gate_up_unit<W, F16, 8>(args, r, buffer, e, i0, tokens);
-    }
+  GateUp<W, F16> g{args, r, ptx::lane_id(), static_cast<int>(threadIdx.x) / 32, (args.I + kCols - 1) / kCols, 0, {}};
+  g.units = *r.count * g.strips;
+  int unit = static_cast<int>(blockIdx.x);
+  if (unit < g.units && g.warp * kMoeStep < args.H) g.load(unit, g.warp * kMoeStep);
+  for (int turn = 0; unit < g.units; unit += static_cast<int>(gridDim.x), turn ^= 1) {
+    const int e = r.list[unit / g.strips];
+    g.run(red + turn * kMoeWarps * stride, stride, unit, e, __popcll(r.mask[e]));
   }
 }
 
 // ------------------------------------------------------------------------------------- down
 // Unit: 16 columns of the output per MMA tile, for all tokens, one cluster. The contraction runs over all
-// chosen experts; its steps go to the warps of the cluster in turn. Column g of n-tile j is token 8 j + g for every
-// expert (zeros where it did not choose it), so the accumulators add the experts up by themselves.
-template <int W, int F16, int NT>
+// chosen experts; its steps go to the warps of the cluster in turn. An expert's tokens are packed into as few tiles
+// as they need; after a step a warp adds its sums to the tokens they belong to, in shared memory of its own
+// (a fixed column per token would need no such sums, but an expert's four tokens among 64 then lie in three or four
+// tiles of eight: 172 us against FIGURE_DOWN for 64 tokens, 128 experts, 2048 x 768).
+template <int W, int F16>
+struct Down {
+  static constexpr int MT = MoeUnit<W>::kTiles;
+  static constexpr int kPitch = MT * 16 + 1;  // floats between tokens
+  using Weights = typename MoeStep<W, F16, 1>::Weights;
+  const MoeArgs& args;
+  const RouteTables& r;
+  uint32_t lane;
+  int r0, steps;
+  Weights w;
+
+  B200_DEVICE void load(int s) {
+    const int e = r.list[s / steps];
+    const int H = args.H, first = r0 + static_cast<int>(lane >> 2);
+    w.load(args.w2, s % steps * kMoeStep, args.I, lane, [=](int m, int half) {
+      const int row = first + m * 16 + half * 8;
+      return row < H ? static_cast<long long>(e) * H + row : -1ll;
+    });
+  }
+
+  // The loaded step against tiles [j0, j0 + NT) of the expert's tokens, on top of the tokens' sums.
+  template <int NT>
+  B200_DEVICE void tiles(float* sums, int first_pair, int tokens, int j0, int k0) {
+    const uint16_t* b[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int c = min((j0 + j) * 8 + static_cast<int>(lane >> 2), tokens - 1);
+      b[j] = args.h + static_cast<long long>(r.pairs[first_pair + c]) * args.I;
+    }
+    float acc[NT][MT][4] = {};
+    MoeStep<W, F16, NT>::mma(w, acc, b, k0, args.I, lane);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int c = (j0 + j) * 8 + static_cast<int>(lane & 3u) * 2 + n;
+        if (c < tokens) {
+          float* to = sums + r.tokens[first_pair + c] * kPitch + (lane >> 2);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            to[m * 16] += acc[j][m][n];
+            to[m * 16 + 8] += acc[j][m][2 + n];
+          }
+        }
+      }
+    }
+  }
+
+  B200_DEVICE void run(float* sums, int s, int next, int total) {
+    const int e = r.list[s / steps];
+    const int tokens = __popcll(r.mask[e]), first_pair = r.first[e];
+    const int n_tiles = (tokens + 7) / 8, k0 = s % steps * kMoeStep;
+    int j = 0;
+    for (; j + 1 < n_tiles; j += 2) tiles<2>(sums, first_pair, tokens, j, k0);
+    if (j < n_tiles) tiles<1>(sums, first_pair, tokens, j, k0);
+    if (next < total) load(next);
+    __syncwarp();  // the next step's lanes may hold other tokens
+  }
+};
+
+template <int W, int F16>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_constant__ MoeArgs args, int split) {
-  constexpr int MT = MoeUnit<W>::kTiles;
+  using D = Down<W, F16>;
   extern __shared__ __align__(16) uint8_t smem[];
-  float4* red = reinterpret_cast<float4*>(smem);
-  const RouteTables r = route_tables_at(smem + kMoeWarps * MT * NT * 32 * 16, args);
-  const uint32_t lane = ptx::lane_id();
+  float* sums = reinterpret_cast<float*>(smem);  // [warp][token][kPitch]
+  const int per_warp = args.T * D::kPitch;
+  const RouteTables r = route_tables_at(smem + (kMoeWarps * per_warp * 4 + 15) / 16 * 16, args);
   const int warp = static_cast<int>(threadIdx.x) / 32;
   const int rank = split > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
-  const int r0 = static_cast<int>(blockIdx.x) / split * 16 * MT;
-  const int g = static_cast<int>(lane >> 2);
+  D d{args, r, ptx::lane_id(), static_cast<int>(blockIdx.x) / split * 16 * D::MT, (args.I + kMoeStep - 1) / kMoeStep, {}};
+  for (int i = static_cast<int>(threadIdx.x); i < kMoeWarps * per_warp; i += kMoeThreads) sums[i] = 0.0f;
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
   build_route_tables(r, args);
-  const int steps = (args.I + kMoeStep - 1) / kMoeStep;
-  const int total = *r.count * steps;
-  float acc[MT][NT][4] = {};
-  for (int s = rank * kMoeWarps + warp; s < total; s += split * kMoeWarps) {
-    const int e = r.list[s / steps];
-    const unsigned long long mask = r.mask[e];
-    const uint16_t* pairs = r.pairs + r.first[e];
-    weight_step<W, F16, NT, MT>(
-        acc, args.w2, s % steps * kMoeStep, args.I, lane,
-        [&](int m, int half) {
-          const int row = r0 + m * 16 + half * 8 + g;
-          return row < args.H ? static_cast<long long>(e) * args.H + row : -1ll;
-        },
-        [&](int j, bool* any) -> const uint16_t* {
-          *any = ((mask >> (8 * j)) & 0xFFull) != 0;
-          const int t = 8 * j + g;
-          if (!((mask >> t) & 1ull)) return nullptr;
-          const int pair = pairs[__popcll(mask & ((1ull << t) - 1ull))];
-          return args.h + static_cast<long long>(pair) * args.I;
-        });
-  }
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      red[((warp * MT + m) * NT + j) * 32 + lane] = make_float4(acc[m][j][0], acc[m][j][1], acc[m][j][2], acc[m][j][3]);
-    }
-  }
+  const int total = *r.count * d.steps, stride = split * kMoeWarps;
+  int s = rank * kMoeWarps + warp;
+  if (s < total) d.load(s);
+  float* mine = sums + warp * per_warp;
+  for (; s < total; s += stride) d.run(mine, s, s + stride, total);
   __syncthreads();
+  // The warps' sums into the first warp's, then the CTAs' into the output, in order.
+  constexpr int kRows = D::MT * 16;
+  for (int i = static_cast<int>(threadIdx.x); i < per_warp; i += kMoeThreads) {
+    float v = sums[i];
+#pragma unroll
+    for (int q = 1; q < kMoeWarps; ++q) v += sums[q * per_warp + i];
+    sums[i] = v;
+  }
   if (split > 1) {
     ptx::cluster_arrive();
     ptx::cluster_wait();
+  } else {
+    __syncthreads();
   }
-  // CTA `rank` finishes its share of the tiles' elements.
-  const uint32_t red_addr = ptx::smem_u32(red);
-  for (int idx = rank * kMoeThreads + static_cast<int>(threadIdx.x); idx < MT * NT * 32; idx += split * kMoeThreads) {
-    float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int p = 0; p < split; ++p) {
-      const uint32_t base = split > 1 ? ptx::map_to_cta(red_addr, static_cast<uint32_t>(p)) : red_addr;
-      for (int q = 0; q < kMoeWarps; ++q) {
-        const float4 v = ptx::ld_cluster_v4(base + static_cast<uint32_t>((q * MT * NT * 32 + idx) * 16));
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
-      }
-    }
-    const int tile = idx / 32;
-    const int row = r0 + tile / NT * 16 + (idx % 32) / 4;
-    const int t = tile % NT * 8 + (idx % 4) * 2;
-    const float lo[2] = {s.x, s.y}, hi[2] = {s.z, s.w};
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      if (t + n < args.T) {
-        uint16_t* o = args.out + static_cast<long long>(t + n) * args.H + row;
-        if (row < args.H) o[0] = round16<F16>(lo[n] * args.lift2);
-        if (row + 8 < args.H) o[8] = round16<F16>(hi[n] * args.lift2);
-      }
-    }
+  const uint32_t addr = ptx::smem_u32(sums);
+  for (int i = rank * kMoeThreads + static_cast<int>(threadIdx.x); i < args.T * kRows; i += split * kMoeThreads) {
+    const int t = i / kRows, row = i % kRows;
+    const uint32_t at = static_cast<uint32_t>((t * D::kPitch + row) * 4);
+    float v = 0.0f;
+#pragma unroll 4
+    for (int p = 0; p < split; ++p) v += ptx::ld_cluster_f32(split > 1 ? ptx::map_to_cta(addr + at, p) : addr + at);
+    if (d.r0 + row < args.H) args.out[static_cast<long long>(t) * args.H + d.r0 + row] = round16<F16>(v * args.lift2);
   }
   if (split > 1) {
     ptx::cluster_arrive();  // no CTA leaves while another reads its sums
