@@ -365,59 +365,51 @@ struct WeightStep {
   }
 };
 
-// What a 4-bit weight's bits are multiplied with. A code's magnitude bits at the top of a bf16 number's mantissa
-// and the bottom of its exponent read code * 2^-126; the factor brings them to code * scale (MXFP4) or
-// code * scale * 2^-16 (NVFP4, whose block scales reach 448: the rest is applied to the sums). MXFP4
-// scales above 2 (byte > 128) need a second factor, 2^(byte - 128); a step without any skips it. Every product is
-// exact in bf16.
-static constexpr float kNvfp4Lift = 65536.0f;
-template <int W>
-B200_DEVICE uint32_t weight_factor(uint32_t byte) {
-  uint32_t f;
-  if constexpr (W == kMoeMxfp4) {
-    f = byte == 255u ? 0x7FC0u : min(byte + 126u, 254u) << 7;
-  } else {
-    f = __float_as_uint(e4m3_value(byte) * 1.298074214633707e33f) >> 16;  // 2^110
-  }
-  return f | (f << 16);
-}
-B200_DEVICE uint32_t weight_second_factor(uint32_t byte) {
-  const uint32_t s = byte > 128u ? (byte - 1u) << 7 : 0x3F80u;
-  return s | (s << 16);
-}
-
 B200_DEVICE uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 
-// 4-bit weights: two chunks of 128 elements, a lane 16 bytes = 32 elements of each row and chunk. Of a word's
-// eight codes, i and i + 4 are 16 bits apart: one shift brings both to their place in a bf16 pair, and B
-// takes its elements in the same order.
+// 4-bit weights: two chunks of 128 elements, a lane 16 bytes = 32 elements of each row and chunk.
+//
+// Unpacking, not memory, is what this kernel spends most instructions on. A code's magnitude bits at the top of a
+// bf16 number's mantissa and the bottom of its exponent read code * 2^-126. Of a word's eight codes, i and
+// i + 4 are 16 bits apart, so a mask, one multiplication (which puts the magnitude at bit 6 and the sign
+// at bit 15 of either half) and a second mask make a bf16 pair of them, and one bf16 multiplication with a
+// factor for the block gives code * scale (MXFP4) or code * scale * 2^-16 (NVFP4, whose scales reach 448: the
+// rest is applied to the sums), exactly. B takes its elements in the same order. The factor of an MXFP4
+// scale above 2 (byte > 128) would leave bf16's range and takes a second one; a step that has any, or a NaN scale,
+// goes the general way.
+static constexpr float kNvfp4Lift = 65536.0f;
 template <int W, int MT>
 struct WeightStep4 {
   static constexpr int FMT = W == kMoeMxfp4 ? kMxfp4 : kNvfp4;
   static constexpr int kBlocks = 32 / mx_block(FMT);  // block scales of a lane's 32 elements
   uint4 q[MT][2][2];
   uint32_t sb[MT][2][2];
-  bool wide;  // a scale needs its second factor
 
   template <typename Rows>
   B200_DEVICE void load(const MoeMatrix& w, int k0, int K, uint32_t lane, Rows rows) {
-    const int part = static_cast<int>(lane & 3u);
+    const uint32_t part = lane & 3u;
+    const uint32_t block = static_cast<uint32_t>(k0) / mx_block(FMT) + part * kBlocks;
+    const uint8_t* codes = w.data + k0 / 2 + part * 16;
+    const uint8_t* scales = w.scales + (block / 4) * kMxGroupBytes + block % 4;
+    const long long tile_row = w.col_tiles * mx_tile_bytes(FMT);
+    const bool live0 = k0 + static_cast<int>(part) * 32 < K, live1 = k0 + 128 + static_cast<int>(part) * 32 < K;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const long long row = rows(m, half);
-        const uint8_t* p = w.data + row * w.pitch + k0 / 2 + part * 16;
-        const uint8_t* sp = w.scales + mx_scale_offset(FMT, row, k0 / mx_block(FMT) + part * kBlocks, w.col_tiles);
+        const long long signed_row = rows(m, half);
+        const uint32_t row = static_cast<uint32_t>(signed_row);  // (at most 512 * 2 * 2^20)
+        const uint8_t* p = codes + row * w.pitch;
+        const uint8_t* sp = scales + (row / kMxTileRows) * tile_row + (row % 32) * 16 + (row % kMxTileRows) / 32 * 4;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           q[m][half][c] = make_uint4(0u, 0u, 0u, 0u);
           sb[m][half][c] = 0u;
-          if (row >= 0 && k0 + c * 128 + part * 32 < K) {
+          if (signed_row >= 0 && (c == 0 ? live0 : live1)) {
             q[m][half][c] = ptx::ld_stream_v4(p + c * 64);
             if constexpr (FMT == kMxfp4) {
               sb[m][half][c] = sp[c * kMxGroupBytes];
@@ -430,52 +422,80 @@ struct WeightStep4 {
     }
   }
 
-  // Codes of word `word` of chunk `c` of one row, as four bf16 pairs.
-  template <bool WIDE>
-  B200_DEVICE void weights(uint32_t (&a)[4], int m, int half, int c, int word) const {
-    const uint4& v = q[m][half][c];
-    const uint32_t codes = word == 0 ? v.x : word == 1 ? v.y : word == 2 ? v.z : v.w;
-    const uint32_t byte = (sb[m][half][c] >> (kBlocks == 2 ? (word / 2) * 8 : 0)) & 0xFFu;
-    const uint32_t f = weight_factor<W>(byte);
+  // The factor of block `i` of a lane's chunk, in both halves, and the second one.
+  template <bool GENERAL>
+  B200_DEVICE void factors(uint32_t bytes, int i, uint32_t* first, uint32_t* second) const {
+    const uint32_t byte = (bytes >> (8 * i)) & 0xFFu;
+    *second = 0x3F803F80u;
+    if constexpr (W == kMoeMxfp4) {
+      if constexpr (GENERAL) {
+        *first = byte == 255u ? 0x7FC07FC0u : min(byte + 126u, 254u) * 0x00800080u;
+        if (byte > 128u) *second = (byte - 1u) * 0x00800080u;  // 2^(byte - 128)
+      } else {
+        *first = byte * 0x00800080u + 126u * 0x00800080u;  // 2^(byte - 1)
+      }
+    } else {
+      // e4m3 bits as a bf16 number are the scale times 2^-120; brought up in two exact steps to 2^110
+      const uint32_t bits = byte * 0x00100010u;
+      *first = mul_bf16x2(mul_bf16x2(bits, 0x7B807B80u), 0x76807680u);
+      if (GENERAL && byte == 0x7Fu) *first = 0x7FC07FC0u;
+    }
+  }
+
+  // Eight codes as four bf16 pairs (i, i + 4).
+  template <bool GENERAL>
+  static B200_DEVICE void unpack(uint32_t (&a)[4], uint32_t codes, uint32_t first, uint32_t second) {
+    const uint32_t upper = codes >> 8;
+    a[0] = ((codes & 0x000F000Fu) * 0x1040u) & 0x81C081C0u;
+    a[1] = ((codes & 0x00F000F0u) * 0x0104u) & 0x81C081C0u;
+    a[2] = ((upper & 0x000F000Fu) * 0x1040u) & 0x81C081C0u;
+    a[3] = ((upper & 0x00F000F0u) * 0x0104u) & 0x81C081C0u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t mag = (i < 2 ? codes << (6 - 4 * i) : codes >> (4 * i - 6)) & 0x01C001C0u;
-      a[i] = mul_bf16x2(mag | ((codes << (12 - 4 * i)) & 0x80008000u), f);
-      if constexpr (WIDE) a[i] = mul_bf16x2(a[i], weight_second_factor(byte));
+      a[i] = mul_bf16x2(a[i], first);
+      if constexpr (GENERAL && W == kMoeMxfp4) a[i] = mul_bf16x2(a[i], second);
     }
   }
 
   // NT n-tiles at once, so that a weight is unpacked once: column g of tile j is the vector b[j].
-  template <int NT, bool WIDE>
+  template <int NT, bool GENERAL>
   B200_DEVICE void mma(float (&acc)[NT][MT][4], const uint16_t* const (&b)[NT], int k0, int K, uint32_t lane) const {
     const int part = static_cast<int>(lane & 3u);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const int kc = k0 + c * 128 + part * 32;
-      const bool live = kc + 32 <= K;
-      uint4 v0[4];
+      uint32_t first[MT][2][kBlocks], second[MT][2][kBlocks];
 #pragma unroll
-      for (int word = 0; word < 4; ++word) {
-        v0[word] = make_uint4(0u, 0u, 0u, 0u);
-        if (live || kc + word * 8 < K) v0[word] = *reinterpret_cast<const uint4*>(b[0] + kc + word * 8);
+      for (int m = 0; m < MT; ++m) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int i = 0; i < kBlocks; ++i) factors<GENERAL>(sb[m][half][c], i, &first[m][half][i], &second[m][half][i]);
+        }
       }
 #pragma unroll
       for (int word = 0; word < 4; ++word) {
+        uint4 v[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          v[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (kc + word * 8 < K) v[j] = *reinterpret_cast<const uint4*>(b[j] + kc + word * 8);
+        }
         uint32_t a[MT][2][4];
+        const int i = kBlocks == 2 ? word / 2 : 0;
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          weights<WIDE>(a[m][0], m, 0, c, word);
-          weights<WIDE>(a[m][1], m, 1, c, word);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint4& w = q[m][half][c];
+            unpack<GENERAL>(a[m][half], word == 0 ? w.x : word == 1 ? w.y : word == 2 ? w.z : w.w, first[m][half][i],
+                            second[m][half][i]);
+          }
         }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          uint4 v = v0[word];
-          if (j > 0) {
-            v = make_uint4(0u, 0u, 0u, 0u);
-            if (kc + word * 8 < K) v = *reinterpret_cast<const uint4*>(b[j] + kc + word * 8);
-          }
-          const uint32_t b0 = __byte_perm(v.x, v.z, 0x5410), b1 = __byte_perm(v.x, v.z, 0x7632);
-          const uint32_t b2 = __byte_perm(v.y, v.w, 0x5410), b3 = __byte_perm(v.y, v.w, 0x7632);
+          const uint32_t b0 = __byte_perm(v[j].x, v[j].z, 0x5410), b1 = __byte_perm(v[j].x, v[j].z, 0x7632);
+          const uint32_t b2 = __byte_perm(v[j].y, v[j].w, 0x5410), b3 = __byte_perm(v[j].y, v[j].w, 0x7632);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             mma16816<0>(acc[j][m], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], b0, b1);
@@ -486,15 +506,21 @@ struct WeightStep4 {
     }
   }
 
-  B200_DEVICE bool needs_second_factor() const {
-    if constexpr (W != kMoeMxfp4) return false;
-    uint32_t most = 0u;
+  B200_DEVICE bool general() const {
+    bool some = false;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) most = max(most, sb[m][i / 2][i % 2]);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t bytes = sb[m][i / 2][i % 2];
+        if constexpr (W == kMoeMxfp4) {
+          some = some || bytes > 128u;
+        } else {
+          some = some || (bytes & 0x7Fu) == 0x7Fu || (bytes & 0x7F00u) == 0x7F00u;
+        }
+      }
     }
-    return __any_sync(0xFFFFFFFFu, most > 128u);
+    return __any_sync(0xFFFFFFFFu, some);
   }
 };
 
@@ -515,7 +541,7 @@ struct MoeStep {
     if constexpr (W == kMoe16) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) w.mma(acc[j], b[j], k0, K, lane);
-    } else if (w.needs_second_factor()) {
+    } else if (w.general()) {
       w.template mma<NT, true>(acc, b, k0, K, lane);
     } else {
       w.template mma<NT, false>(acc, b, k0, K, lane);
