@@ -321,7 +321,7 @@ struct WeightStep {
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const long long row = rows(m, half);
+        const int row = rows(m, half);
         const uint8_t* p = w.data + row * w.pitch + kl * 2;
         if (row >= 0 && k0 + kMoeStep <= K) {
 #pragma unroll
@@ -401,8 +401,8 @@ struct WeightStep4 {
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const long long signed_row = rows(m, half);
-        const uint32_t row = static_cast<uint32_t>(signed_row);  // (at most 512 * 2 * 2^20)
+        const int signed_row = rows(m, half);
+        const uint32_t row = static_cast<uint32_t>(signed_row);
         const uint8_t* p = codes + row * w.pitch;
         const uint8_t* sp = scales + (row / kMxTileRows) * tile_row + (row % 32) * 16 + (row % kMxTileRows) / 32 * 4;
 #pragma unroll
@@ -457,7 +457,8 @@ struct WeightStep4 {
     }
   }
 
-  // NT n-tiles at once, so that a weight is unpacked once: column g of tile j is the vector b[j].
+  // NT n-tiles at once, so that a weight is unpacked once: column g of tile j is the vector b[j]. GENERAL: any
+  // scale, and a step that the end of the rows may cut short.
   template <int NT, bool GENERAL>
   B200_DEVICE void mma(float (&acc)[NT][MT][4], const uint16_t* const (&b)[NT], int k0, int K, uint32_t lane) const {
     const int part = static_cast<int>(lane & 3u);
@@ -478,8 +479,8 @@ struct WeightStep4 {
         uint4 v[NT];
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          v[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (kc + word * 8 < K) v[j] = *reinterpret_cast<const uint4*>(b[j] + kc + word * 8);
+          if constexpr (GENERAL) v[j] = make_uint4(0u, 0u, 0u, 0u);
+          if (!GENERAL || kc + word * 8 < K) v[j] = *reinterpret_cast<const uint4*>(b[j] + kc + word * 8);
         }
         uint32_t a[MT][2][4];
         const int i = kBlocks == 2 ? word / 2 : 0;
@@ -541,7 +542,7 @@ struct MoeStep {
     if constexpr (W == kMoe16) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) w.mma(acc[j], b[j], k0, K, lane);
-    } else if (w.general()) {
+    } else if (k0 + kMoeStep > K || w.general()) {
       w.template mma<NT, true>(acc, b, k0, K, lane);
     } else {
       w.template mma<NT, false>(acc, b, k0, K, lane);
@@ -559,6 +560,18 @@ B200_DEVICE float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
 // a lane ends up with a gate value and its up value. The CTAs take units in turn; a warp issues the next
 // step's loads, of the next unit if need be, as soon as its MMAs have taken the registers, so that memory is busy
 // while the sums are joined.
+struct UnitCursor {
+  int index, strip;  // chosen expert, strip of its columns
+  B200_DEVICE void advance(int strips, int by_index, int by_strip) {
+    index += by_index;
+    strip += by_strip;
+    if (strip >= strips) {
+      strip -= strips;
+      ++index;
+    }
+  }
+};
+
 template <int W, int F16>
 struct GateUp {
   static constexpr int MT = MoeUnit<W>::kTiles;
@@ -567,16 +580,13 @@ struct GateUp {
   const MoeArgs& args;
   const RouteTables& r;
   uint32_t lane;
-  int warp, strips, units;
+  int warp, experts;
   Weights w;
 
-  B200_DEVICE void load(int unit, int k0) {
-    const int e = r.list[unit / strips];
-    const int i0 = unit % strips * kCols;
-    const long long row = static_cast<long long>(e) * 2 * args.I + i0 + (lane >> 2);
-    const int I = args.I;
-    w.load(args.w1, k0, args.H, lane,
-           [=](int m, int half) { return i0 + m * 8 < I ? row + m * 8 + (half ? I : 0) : -1ll; });
+  B200_DEVICE void load(const UnitCursor& u, int k0) {
+    const int I = args.I, i0 = u.strip * kCols;
+    const int row = r.list[u.index] * 2 * I + i0 + static_cast<int>(lane >> 2);
+    w.load(args.w1, k0, args.H, lane, [=](int m, int half) { return m == 0 || i0 + m * 8 < I ? row + m * 8 + (half ? I : 0) : -1; });
   }
 
   // The loaded step against tiles [j0, j0 + NT) of the unit's tokens; sums go to (first) or on top of `mine`.
@@ -609,50 +619,49 @@ struct GateUp {
   }
 
   // `red`: every warp's sums, `stride` float4 apart.
-  B200_DEVICE void run(float4* red, int stride, int unit, int e, int tokens) {
-    const int first_pair = r.first[e];
+  B200_DEVICE void run(float4* red, int stride, const UnitCursor& unit, const UnitCursor& next) {
+    const int e = r.list[unit.index];
+    const int tokens = __popcll(r.mask[e]), first_pair = r.first[e];
     const int n_tiles = (tokens + 7) / 8;
+    const int own = warp * kMoeStep;
     float4* mine = red + warp * stride;
-    for (int k0 = warp * kMoeStep; k0 - warp * kMoeStep < args.H; k0 += kMoeWarps * kMoeStep) {
-      const bool first = k0 == warp * kMoeStep;
+    for (int k0 = own; k0 - own < args.H; k0 += kMoeWarps * kMoeStep) {
       if (k0 < args.H) {
         int j = 0;
-        for (; j + 1 < n_tiles; j += 2) tiles<2>(mine, first_pair, tokens, j, k0, first);
-        if (j < n_tiles) tiles<1>(mine, first_pair, tokens, j, k0, first);
-      } else if (first) {
+        for (; j + 1 < n_tiles; j += 2) tiles<2>(mine, first_pair, tokens, j, k0, k0 == own);
+        if (j < n_tiles) tiles<1>(mine, first_pair, tokens, j, k0, k0 == own);
+      } else if (k0 == own) {
         for (int i = 0; i < n_tiles * MT; ++i) mine[i * 32 + lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
       const int k_next = k0 + kMoeWarps * kMoeStep;
-      if (k_next - warp * kMoeStep < args.H) {
+      if (k_next - own < args.H) {
         if (k_next < args.H) load(unit, k_next);
-      } else if (unit + static_cast<int>(gridDim.x) < units && warp * kMoeStep < args.H) {
-        load(unit + static_cast<int>(gridDim.x), warp * kMoeStep);
+      } else if (next.index < experts && own < args.H) {
+        load(next, own);
       }
     }
     __syncthreads();
-    // Four threads per hidden value, two warps' sums each.
-    const int i0 = unit % strips * kCols;
-    const int quarter = static_cast<int>(threadIdx.x) & 3;
-    for (int o = static_cast<int>(threadIdx.x) / 4; o < n_tiles * MT * 64; o += kMoeThreads / 4) {
+    const int i0 = unit.strip * kCols;
+    for (int o = static_cast<int>(threadIdx.x); o < n_tiles * MT * 64; o += kMoeThreads) {
       const int tile = o / 64, row_in = o % 64 / 8, col = o % 8;
-      const float* at = reinterpret_cast<const float*>(red + 2 * quarter * stride + tile * 32 + row_in * 4 + col / 2) + (col & 1);
-      float gate = at[0] + at[stride * 4], up = at[2] + at[stride * 4 + 2];
-      gate += __shfl_xor_sync(0xFFFFFFFFu, gate, 1);
-      up += __shfl_xor_sync(0xFFFFFFFFu, up, 1);
-      gate += __shfl_xor_sync(0xFFFFFFFFu, gate, 2);
-      up += __shfl_xor_sync(0xFFFFFFFFu, up, 2);
       const int c = tile / MT * 8 + col, row = i0 + tile % MT * 8 + row_in;
-      if (quarter == 0 && c < tokens && row < args.I) {
-        args.h[static_cast<long long>(r.pairs[first_pair + c]) * args.I + row] =
-            round16<F16>(r.weights[first_pair + c] * (silu(gate * args.lift1) * (up * args.lift1)));
+      if (c >= tokens || row >= args.I) continue;
+      const float* at = reinterpret_cast<const float*>(red + tile * 32 + row_in * 4 + col / 2) + (col & 1);
+      float gate = at[0], up = at[2];
+#pragma unroll
+      for (int p = 1; p < kMoeWarps; ++p) {
+        gate += at[p * stride * 4];
+        up += at[p * stride * 4 + 2];
       }
+      args.h[static_cast<long long>(r.pairs[first_pair + c]) * args.I + row] =
+          round16<F16>(r.weights[first_pair + c] * (silu(gate * args.lift1) * (up * args.lift1)));
     }
   }
 };
 
 __host__ __device__ __forceinline__ int moe_token_tiles(int T) { return (T + 7) / 8; }
-// float4 between two warps' sums: the padding keeps the four threads of a value on different banks.
-__host__ __device__ __forceinline__ int gate_up_stride(int tiles, int T) { return tiles * moe_token_tiles(T) * 32 + 2; }
+// float4 between two warps' sums
+__host__ __device__ __forceinline__ int gate_up_stride(int tiles, int T) { return tiles * moe_token_tiles(T) * 32; }
 
 template <int W, int F16>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __grid_constant__ MoeArgs args) {
@@ -662,15 +671,18 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __gri
   const int stride = gate_up_stride(MoeUnit<W>::kTiles, args.T);
   const RouteTables r = route_tables_at(smem + 2 * kMoeWarps * stride * 16, args);
   ptx::grid_launch_dependents();
+  const int strips = (args.I + kCols - 1) / kCols;
+  const int by_index = static_cast<int>(gridDim.x) / strips, by_strip = static_cast<int>(gridDim.x) % strips;
+  UnitCursor unit{static_cast<int>(blockIdx.x) / strips, static_cast<int>(blockIdx.x) % strips};
   ptx::grid_dependency_wait();
   build_route_tables(r, args);
-  GateUp<W, F16> g{args, r, ptx::lane_id(), static_cast<int>(threadIdx.x) / 32, (args.I + kCols - 1) / kCols, 0, {}};
-  g.units = *r.count * g.strips;
-  int unit = static_cast<int>(blockIdx.x);
-  if (unit < g.units && g.warp * kMoeStep < args.H) g.load(unit, g.warp * kMoeStep);
-  for (int turn = 0; unit < g.units; unit += static_cast<int>(gridDim.x), turn ^= 1) {
-    const int e = r.list[unit / g.strips];
-    g.run(red + turn * kMoeWarps * stride, stride, unit, e, __popcll(r.mask[e]));
+  GateUp<W, F16> g{args, r, ptx::lane_id(), static_cast<int>(threadIdx.x) / 32, *r.count, {}};
+  if (unit.index < g.experts && g.warp * kMoeStep < args.H) g.load(unit, g.warp * kMoeStep);
+  for (int turn = 0; unit.index < g.experts; turn ^= 1) {
+    UnitCursor next = unit;
+    next.advance(strips, by_index, by_strip);
+    g.run(red + turn * kMoeWarps * stride, stride, unit, next);
+    unit = next;
   }
 }
 
@@ -696,7 +708,7 @@ struct Down {
     const int H = args.H, first = r0 + static_cast<int>(lane >> 2);
     w.load(args.w2, s % steps * kMoeStep, args.I, lane, [=](int m, int half) {
       const int row = first + m * 16 + half * 8;
-      return row < H ? static_cast<long long>(e) * H + row : -1ll;
+      return row < H ? e * H + row : -1;
     });
   }
 
