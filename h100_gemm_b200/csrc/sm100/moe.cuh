@@ -234,19 +234,19 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid
 
 // ------------------------------------------------------------------------------------- routing tables
 // What a CTA of the two product kernels knows of the routing, built from ids by itself: the experts
-// anybody chose, the tokens of each as a bit mask, and the (token, choice) pairs ordered by
-// expert and token.
+// anybody chose in ascending order, and the (token, choice) pairs ordered by expert and token.
 struct RouteTables {
-  unsigned long long* mask;  // [E]
+  unsigned long long* mask;  // [E] tokens of an expert (while the tables are built)
   float* weights;            // routing weight of a pair
-  uint16_t* pairs;           // [T * k] token * k + choice
-  uint16_t* list;            // [E] chosen experts, ascending
-  uint16_t* first;           // [E] first pair of an expert in `pairs`
-  uint8_t* tokens;           // token of a pair
   int* count;                // chosen experts
+  uint16_t* pairs;           // [T * k] token * k + choice
+  uint16_t* list;            // [E] chosen experts
+  uint16_t* first;           // [E] their first pairs (while the tables are built: by expert)
+  uint8_t* tokens;           // token of a pair
+  uint8_t* size;             // [E] tokens of a chosen expert
 };
 
-__host__ __device__ __forceinline__ int route_table_bytes(int E, int pairs) { return (E * 12 + pairs * 7 + 16 + 15) / 16 * 16; }
+__host__ __device__ __forceinline__ int route_table_bytes(int E, int pairs) { return (E * 13 + pairs * 7 + 16 + 15) / 16 * 16; }
 
 B200_DEVICE RouteTables route_tables_at(uint8_t* smem, const MoeArgs& args) {
   const int pairs = args.T * args.k;
@@ -258,17 +258,65 @@ B200_DEVICE RouteTables route_tables_at(uint8_t* smem, const MoeArgs& args) {
   r.list = r.pairs + pairs;
   r.first = r.list + args.E;
   r.tokens = reinterpret_cast<uint8_t*>(r.first + args.E);
+  r.size = r.tokens + pairs;
   return r;
+}
+
+// Up to 32 pairs, a decode step of one to a few tokens: one warp, a lane a pair, every lane compared with every other.
+B200_DEVICE void build_small_route_tables(const RouteTables& r, const MoeArgs& args) {
+  const int lane = static_cast<int>(threadIdx.x);
+  if (lane < 32) {
+    const int pairs = args.T * args.k;
+    const int e = lane < pairs ? __ldcg(args.ids + lane) : -1;
+    const float weight = e >= 0 ? __ldcg(args.weights + lane) : 0.0f;
+    int before = 0, same = 0, same_before = 0;
+    for (int q = 0; q < pairs; ++q) {
+      const int other = __shfl_sync(0xFFFFFFFFu, e, q);
+      before += other >= 0 && other < e;
+      same += other == e;
+      same_before += other == e && q < lane;
+    }
+    const bool head = e >= 0 && same_before == 0;
+    int index = 0;  // chosen experts before this one
+    for (int q = 0; q < pairs; ++q) {
+      const int other = __shfl_sync(0xFFFFFFFFu, head ? e : 0x7FFFFFFF, q);
+      index += other < e;
+    }
+    if (e >= 0) {
+      r.pairs[before + same_before] = static_cast<uint16_t>(lane);
+      r.tokens[before + same_before] = static_cast<uint8_t>(lane / args.k);
+      r.weights[before + same_before] = weight;
+    }
+    if (head) {
+      r.list[index] = static_cast<uint16_t>(e);
+      r.first[index] = static_cast<uint16_t>(before);
+      r.size[index] = static_cast<uint8_t>(same);
+    }
+    const uint32_t heads = __ballot_sync(0xFFFFFFFFu, head);
+    if (lane == 0) *r.count = __popc(heads);
+  }
+  __syncthreads();
 }
 
 B200_DEVICE void build_route_tables(const RouteTables& r, const MoeArgs& args) {
   const int t = static_cast<int>(threadIdx.x);
   const int pairs = args.T * args.k;
+  if (pairs <= 32) {
+    build_small_route_tables(r, args);
+    return;
+  }
+  constexpr int kPer = kMoeMaxTokens * kMoeMaxTopK / kMoeThreads;  // pairs of a thread, kept for the second pass
+  int mine[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int p = t + i * kMoeThreads;
+    mine[i] = p < pairs ? __ldcg(args.ids + p) : -1;
+  }
   for (int e = t; e < args.E; e += kMoeThreads) r.mask[e] = 0ull;
   __syncthreads();
-  for (int p = t; p < pairs; p += kMoeThreads) {
-    const int e = __ldcg(args.ids + p);
-    if (e >= 0) atomicOr(r.mask + e, 1ull << (p / args.k));
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    if (mine[i] >= 0) atomicOr(r.mask + mine[i], 1ull << ((t + i * kMoeThreads) / args.k));
   }
   __syncthreads();
   if (t < 32) {
@@ -284,21 +332,37 @@ B200_DEVICE void build_route_tables(const RouteTables& r, const MoeArgs& args) {
         if (t >= d) before += other;
       }
       if (e < args.E) r.first[e] = static_cast<uint16_t>(base + before - n);
-      if (n > 0) r.list[found + __popc(some & ((1u << t) - 1u))] = static_cast<uint16_t>(e);
+      if (n > 0) {
+        const int index = found + __popc(some & ((1u << t) - 1u));
+        r.list[index] = static_cast<uint16_t>(e);
+        r.size[index] = static_cast<uint8_t>(n);
+      }
       found += __popc(some);
       base += __shfl_sync(0xFFFFFFFFu, before, 31);
     }
     if (t == 0) *r.count = found;
   }
   __syncthreads();
-  for (int p = t; p < pairs; p += kMoeThreads) {
-    const int e = __ldcg(args.ids + p);
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = mine[i], p = t + i * kMoeThreads;
     if (e >= 0) {
       const int token = p / args.k;
       const int at = r.first[e] + __popcll(r.mask[e] & ((1ull << token) - 1ull));
       r.pairs[at] = static_cast<uint16_t>(p);
       r.tokens[at] = static_cast<uint8_t>(token);
       r.weights[at] = __ldcg(args.weights + p);
+    }
+  }
+  __syncthreads();
+  // From by expert to by position: position i's expert is not before i, so going up overwrites nothing still to be read.
+  if (t < 32) {
+    for (int i0 = 0; i0 < *r.count; i0 += 32) {
+      const int i = i0 + t;
+      const uint16_t first = i < *r.count ? r.first[r.list[i]] : 0;
+      __syncwarp();
+      if (i < *r.count) r.first[i] = first;
+      __syncwarp();
     }
   }
   __syncthreads();
@@ -620,8 +684,7 @@ struct GateUp {
 
   // `red`: every warp's sums, `stride` float4 apart.
   B200_DEVICE void run(float4* red, int stride, const UnitCursor& unit, const UnitCursor& next) {
-    const int e = r.list[unit.index];
-    const int tokens = __popcll(r.mask[e]), first_pair = r.first[e];
+    const int tokens = r.size[unit.index], first_pair = r.first[unit.index];
     const int n_tiles = (tokens + 7) / 8;
     const int own = warp * kMoeStep;
     float4* mine = red + warp * stride;
@@ -741,8 +804,7 @@ struct Down {
   }
 
   B200_DEVICE void run(float* sums, int s, int next, int total) {
-    const int e = r.list[s / steps];
-    const int tokens = __popcll(r.mask[e]), first_pair = r.first[e];
+    const int tokens = r.size[s / steps], first_pair = r.first[s / steps];
     const int n_tiles = (tokens + 7) / 8, k0 = s % steps * kMoeStep;
     int j = 0;
     for (; j + 1 < n_tiles; j += 2) tiles<2>(sums, first_pair, tokens, j, k0);

@@ -6,9 +6,10 @@
 //   code    = RN_e2m1(x / scale), ties to even, saturating at 6; s = 0 gives zeros
 //   a block that holds a NaN or an infinity gets the NaN scale (and zero codes)
 // Everything is exact for 16-bit inputs. Division by 2^e is. For NVFP4, x / t has at most 11
-// significant bits and a border between two codes times s at most 7, so a quotient that is not on a border
-// differs from it by 2^-11 relative or more; x * RN(1 / s) is within 2^-23 of the quotient and,
-// rounded to 12 bits, on the border exactly when the quotient is.
+// significant bits and a border between two codes (0.25 or more) times s at most 7, so a quotient x / (s t) that is
+// not on a border is 2^-13 away from it or more. x * (1 / (s t)) with a reciprocal good to 2^-22 is within 2^-19 of
+// the quotient, and rounded to a multiple of 2^-14 it lies on the border exactly when the quotient does.
+// Likewise a / (6 t): rounded to 12 significant bits before it becomes an e4m3 number of four.
 //
 // Bound by memory: 2 bytes read and 0.53 (MXFP4) or 0.56 (NVFP4) written per element and direction. A CTA
 // takes 128 x 128 elements: 256 bytes of every row (whole lines), eight 16-byte loads in flight per
@@ -51,6 +52,24 @@ __device__ __forceinline__ float half_bits_to_float(uint32_t bits) {
   }
 }
 
+// Elements [lo, hi) of the eight at src, the others zero.
+__device__ __forceinline__ void load_elements(uint32_t (&w)[4], const uint16_t* src, int lo, int hi) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j >= lo && j < hi) w[j / 2] |= static_cast<uint32_t>(src[j]) << (16 * (j & 1));
+  }
+}
+
+// Eight 16-bit elements from element `at` of a row in shared memory (the row itself starts on 4 bytes).
+__device__ __forceinline__ void read_shifted(uint32_t (&w)[4], const uint8_t* row, int at) {
+  const uint32_t* words = reinterpret_cast<const uint32_t*>(row) + (at >> 1);
+  uint32_t v[5];
+#pragma unroll
+  for (int k = 0; k < 5; ++k) v[k] = (k < 4 || (at & 1)) ? words[k] : 0u;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) w[k] = (at & 1) ? __funnelshift_r(v[k], v[k + 1], 16) : v[k];
+}
+
 // The block's scale byte and what its elements are multiplied with; `amax` = largest magnitude as bits.
 // clip > 0 asks for the elements to be clipped to it first (the product would leave fp32's range).
 template <int FMT, int F16>
@@ -66,10 +85,14 @@ __device__ __forceinline__ void block_scale(uint32_t amax, float inv_t, uint32_t
     *mult = __uint_as_float((254u - b) << 23);
   } else {
     const float scaled = a * inv_t;
-    const uint32_t b = e4m3_byte(__fdiv_rn(scaled, 6.0f));
-    *byte = *bad ? 127u : b;
-    *mult = b == 0u ? 0.0f : __frcp_rn(e4m3_value(b));
     *saturated = scaled > 2688.0f;
+    const float sixth = fminf(scaled, 2688.0f) * (1.0f / 6.0f);
+    const float c = sixth * 4097.0f;
+    const uint32_t b = e4m3_byte(__fsub_rn(c, __fsub_rn(c, sixth)));
+    *byte = *bad ? 127u : b;
+    float r;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(e4m3_value(b)));
+    *mult = b == 0u ? 0.0f : r;
   }
 }
 
@@ -80,19 +103,16 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], float inv_
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     v[j] = half_bits_to_float<F16>((j & 1) ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu);
-    if constexpr (FMT == kNvfp4) v[j] *= inv_t;
   }
   if constexpr (FMT == kNvfp4) {
     if (saturated) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j], -2688.0f), 2688.0f);
+      for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j] * inv_t, -2688.0f), 2688.0f);
     }
+    const float m = saturated ? mult : mult * inv_t;
+    constexpr float kRound = 768.0f;  // numbers from 512 to 1024 are multiples of 2^-14
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float y = v[j] * mult;
-      const float c = y * 4097.0f;  // round to 12 significant bits
-      v[j] = __fsub_rn(c, __fsub_rn(c, y));
-    }
+    for (int j = 0; j < 8; ++j) v[j] = __fsub_rn(__fmaf_rn(v[j], m, kRound), kRound);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= mult;
@@ -105,7 +125,7 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], float inv_
 template <int FMT, int F16, int ROW, int COL, int VEC>
 __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_constant__ QuantArgs args) {
   constexpr int kGroups = kQuantTile / (4 * mx_block(FMT));  // scale groups of this tile: 1 or 2
-  __shared__ __align__(16) uint8_t tile[COL ? kQuantTile * kQuantPitch : 16];
+  __shared__ __align__(16) uint8_t tile[COL || !VEC ? kQuantTile * kQuantPitch : 16];
   __shared__ __align__(16) uint8_t scale_row[ROW ? kGroups * kMxGroupBytes : 16];
   __shared__ __align__(16) uint8_t scale_col[COL ? kGroups * kMxGroupBytes : 16];
   const int t = static_cast<int>(threadIdx.x);
@@ -117,25 +137,65 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_co
   ptx::grid_dependency_wait();
 
   uint32_t w[8][4];
+  if constexpr (VEC) {
 #pragma unroll
-  for (int p = 0; p < 8; ++p) {
-    const long long row = r0 + p * 16 + (t >> 4);
-    w[p][0] = w[p][1] = w[p][2] = w[p][3] = 0u;
-    if (row < args.rows) {
-      const uint16_t* src = args.x + row * args.ldx + col;
-      if (VEC && col + 8 <= args.cols) {
-        const uint4 q = ptx::ld_stream_v4(src);
-        w[p][0] = q.x;
-        w[p][1] = q.y;
-        w[p][2] = q.z;
-        w[p][3] = q.w;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (col + j < args.cols) w[p][j / 2] |= static_cast<uint32_t>(src[j]) << (16 * (j & 1));
+    for (int p = 0; p < 8; ++p) {
+      const long long row = r0 + p * 16 + (t >> 4);
+      w[p][0] = w[p][1] = w[p][2] = w[p][3] = 0u;
+      if (row < args.rows) {
+        const uint16_t* src = args.x + row * args.ldx + col;
+        if (col + 8 <= args.cols) {
+          const uint4 q = ptx::ld_stream_v4(src);
+          w[p][0] = q.x;
+          w[p][1] = q.y;
+          w[p][2] = q.z;
+          w[p][3] = q.w;
+        } else {
+          load_elements(w[p], src, 0, static_cast<int>(args.cols - col));
         }
       }
     }
+  } else {
+    // Rows off 16 bytes: the aligned pieces that cover a row of the tile go to shared memory as they lie, and
+    // every thread takes its eight elements from there (element by element the loads took three times as long).
+    uint4 piece_data[9];
+    const int lane16 = t & 15;
+#pragma unroll
+    for (int p = 0; p < 9; ++p) {
+      // (eight passes of 16 pieces, then the seventeenth pieces of all rows)
+      const int r = p < 8 ? p * 16 + (t >> 4) : t;
+      const int k = p < 8 ? lane16 : 16;
+      const long long row = r0 + r;
+      uint32_t e[4] = {0u, 0u, 0u, 0u};
+      if (r < kQuantTile && row < args.rows) {
+        const uint16_t* src = args.x + row * args.ldx + c0;
+        const int from = k * 8 - static_cast<int>(reinterpret_cast<uintptr_t>(src) & 15u) / 2;  // of the tile's columns
+        if (c0 + from >= 0 && c0 + from + 8 <= args.cols) {
+          const uint4 q = ptx::ld_stream_v4(src + from);
+          e[0] = q.x;
+          e[1] = q.y;
+          e[2] = q.z;
+          e[3] = q.w;
+        } else {
+          const long long lo = -(c0 + from), hi = args.cols - (c0 + from);
+          load_elements(e, src + from, lo > 0 ? static_cast<int>(lo) : 0, hi < 8 ? static_cast<int>(hi) : 8);
+        }
+      }
+      piece_data[p] = make_uint4(e[0], e[1], e[2], e[3]);
+    }
+#pragma unroll
+    for (int p = 0; p < 9; ++p) {
+      const int r = p < 8 ? p * 16 + (t >> 4) : t;
+      if (r < kQuantTile) *reinterpret_cast<uint4*>(tile + r * kQuantPitch + (p < 8 ? lane16 : 16) * 16) = piece_data[p];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+      const int r = p * 16 + (t >> 4);
+      const int lead = static_cast<int>(reinterpret_cast<uintptr_t>(args.x + (r0 + r) * args.ldx + c0) & 15u) / 2;
+      read_shifted(w[p], tile + r * kQuantPitch, piece * 8 + lead);
+    }
+    if constexpr (COL) __syncthreads();  // (the tile takes the same elements again, in place)
   }
 
   if constexpr (COL) {
@@ -251,15 +311,15 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_
   const int t = static_cast<int>(threadIdx.x);
   const long long tx = blockIdx.x % args.tiles_x, ty = blockIdx.x / args.tiles_x;
   const long long col = tx * kQuantTile + (t & 15) * 8;
+  __shared__ __align__(16) uint8_t tile[VEC ? 16 : kQuantTile * kQuantPitch];
   ptx::grid_launch_dependents();
   ptx::grid_dependency_wait();
-  if (col >= args.cols) return;
   uint32_t codes[8], byte[8];
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
     const long long row = ty * kQuantTile + p * 16 + (t >> 4);
     codes[p] = byte[p] = 0u;
-    if (row < args.rows) {
+    if (row < args.rows && col < args.cols) {
       codes[p] = *reinterpret_cast<const uint32_t*>(args.data + row * args.pitch + col / 2);
       byte[p] = args.scales[mx_scale_offset(FMT, row, col / mx_block(FMT), args.col_tiles)];
     }
@@ -267,7 +327,7 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_
 #pragma unroll
   for (int p = 0; p < 8; ++p) {
     const long long row = ty * kQuantTile + p * 16 + (t >> 4);
-    if (row >= args.rows) continue;
+    if (row >= args.rows || col >= args.cols) continue;
     const float scale = mx_scale_value<FMT>(byte[p]);
     uint32_t w[4];
 #pragma unroll
@@ -280,13 +340,51 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_
         asm("cvt.rn.bf16x2.f32 %0, %2, %1;" : "=r"(w[j]) : "f"(lo), "f"(hi));
       }
     }
-    uint16_t* dst = args.x + row * args.ldx + col;
-    if (VEC && col + 8 <= args.cols) {
-      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
+    if constexpr (VEC) {
+      uint16_t* dst = args.x + row * args.ldx + col;
+      if (col + 8 <= args.cols) {
+        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (col + j < args.cols) dst[j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+        for (int j = 0; j < 8; ++j) {
+          if (col + j < args.cols) dst[j] = static_cast<uint16_t>(w[j / 2] >> (16 * (j & 1)));
+        }
+      }
+    } else {
+      *reinterpret_cast<uint4*>(tile + (p * 16 + (t >> 4)) * kQuantPitch + (t & 15) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  if constexpr (!VEC) {
+    // Rows off 16 bytes: whole aligned pieces of x by 16 threads per row, then what lies before and after them
+    // (element by element, 4999 x 5005 took 79 us).
+    __syncthreads();
+    const long long c0 = tx * kQuantTile;
+    const int cols = static_cast<int>(args.cols - c0 < kQuantTile ? args.cols - c0 : kQuantTile);
+    auto head_of = [&](const uint16_t* dst) {
+      const int head = static_cast<int>((16u - (reinterpret_cast<uintptr_t>(dst) & 15u)) & 15u) / 2;
+      return head < cols ? head : cols;
+    };
+#pragma unroll 4
+    for (int p = 0; p < 8; ++p) {
+      const int r = p * 16 + (t >> 4);
+      const long long row = ty * kQuantTile + r;
+      if (row >= args.rows) break;
+      uint16_t* dst = args.x + row * args.ldx + c0;
+      const int e = head_of(dst) + (t & 15) * 8;
+      if (e + 8 > cols) continue;
+      uint32_t v[4];
+      read_shifted(v, tile + r * kQuantPitch, e);
+      *reinterpret_cast<uint4*>(dst + e) = make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    const long long row = ty * kQuantTile + (t & 127);
+    if (row < args.rows) {
+      uint16_t* dst = args.x + row * args.ldx + c0;
+      const uint16_t* src = reinterpret_cast<const uint16_t*>(tile + (t & 127) * kQuantPitch);
+      const int head = head_of(dst), tail = head + (cols - head) / 8 * 8;
+      if (t < 128) {
+        for (int k = 0; k < head; ++k) dst[k] = src[k];
+      } else {
+        for (int k = tail; k < cols; ++k) dst[k] = src[k];
       }
     }
   }

@@ -55,22 +55,27 @@ def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: 
             raise _invalid(f"w_gate_up must be [{E}, 2 I, {H}] and w_down [{E}, {H}, I]")
     if H % 8 or I % 8 or H == 0 or I == 0:
         raise _invalid("hidden and inner sizes must be multiples of 8")
-    device = x.device
+    device, dtype = x.device, x.dtype
     _require_cuda(device, "x")
-    for name, t, dtype in (("x", x, x.dtype), ("router", router, x.dtype), ("bias", bias, torch.float32),
-                           ("w_gate_up", None if four_bit else w_gate_up, x.dtype),
-                           ("w_down", None if four_bit else w_down, x.dtype)):
-        if t is None:
-            continue
-        _require_cuda(t.device, name, device)
+
+    def pointer(t, name, dtype, align=16):
+        if t.device != device:
+            _require_cuda(t.device, name, device)
         if t.dtype is not dtype or not t.is_contiguous():
             raise _invalid(f"{name} must be a contiguous {dtype} tensor")
-        if t is not bias and t.data_ptr() % 16:
-            raise _invalid(f"{name} must start on 16 bytes")
-    if bias is not None and tuple(bias.shape) != (E,):
-        raise _invalid(f"bias must have shape ({E},)")
+        p = t.data_ptr()
+        if p % align:
+            raise _invalid(f"{name} must start on {align} bytes")
+        return p
+
+    x_ptr, router_ptr = pointer(x, "x", dtype), pointer(router, "router", dtype)
+    bias_ptr = None
+    if bias is not None:
+        if bias.shape != (E,):
+            raise _invalid(f"bias must have shape ({E},)")
+        bias_ptr = pointer(bias, "bias", torch.float32, 4)
     if out is not None:
-        _output(out, (T, H), x.dtype, device, True)
+        _output(out, (T, H), dtype, device, True)
     need = moe_workspace_bytes(T, E, top_k, H, I)
     if workspace is not None:
         _require_cuda(workspace.device, "workspace", device)
@@ -82,17 +87,19 @@ def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: 
         w1 = (FORMATS[w_gate_up.format], w_gate_up._data_ptr, w_gate_up._scales_ptr, w_gate_up.tensor_scale)
         w2 = (w_down._data_ptr, w_down._scales_ptr, w_down.tensor_scale)
     else:
-        w1, w2 = (-1, w_gate_up.data_ptr(), None, 1.0), (w_down.data_ptr(), None, 1.0)
+        w1 = (-1, pointer(w_gate_up, "w_gate_up", dtype), None, 1.0)
+        w2 = (pointer(w_down, "w_down", dtype), None, 1.0)
 
     def body(handle):
-        y = out if out is not None else torch.empty((T, H), dtype=x.dtype, device=device)
+        y = out if out is not None else torch.empty_like(x)
         ws = workspace if workspace is not None else torch.empty(need, dtype=torch.uint8, device=device)
-        ids = torch.empty((T, top_k), dtype=torch.int32, device=device) if return_routing else None
-        weights = torch.empty((T, top_k), dtype=torch.float32, device=device) if return_routing else None
-        rc = api.library().b200_moe_layer(
-            f16, T, E, top_k, H, I, x.data_ptr(), router.data_ptr(), bias.data_ptr() if bias is not None else None, *w1,
-            *w2, 1 if renormalize else 0, y.data_ptr(), ids.data_ptr() if return_routing else None,
-            weights.data_ptr() if return_routing else None, ws.data_ptr(), need, handle)
+        ids = weights = ids_ptr = weights_ptr = None
+        if return_routing:
+            ids = torch.empty((T, top_k), dtype=torch.int32, device=device)
+            weights = torch.empty((T, top_k), dtype=torch.float32, device=device)
+            ids_ptr, weights_ptr = ids.data_ptr(), weights.data_ptr()
+        rc = api.library().b200_moe_layer(f16, T, E, top_k, H, I, x_ptr, router_ptr, bias_ptr, *w1, *w2, 1 if renormalize else 0,
+                                          y.data_ptr(), ids_ptr, weights_ptr, ws.data_ptr(), need, handle)
         if rc:
             api._check(rc)
         return (y, ids, weights) if return_routing else y

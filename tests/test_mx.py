@@ -472,3 +472,59 @@ def test_product_many_tiles(M, N, K, fmt):
     assert bad == 0, f"{bad} of {M * N} outside"
     assert torch.equal(out, g.gemm_mx(a, b))
     assert g.device_status()[0] == api.STATUS_OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_quantise_borders_of_every_scale(fmt, dtype):
+    """Every border between two codes, exactly and one step of the type to either side, under every scale a block
+    can have: a block's largest magnitude decides the scale, the borders of that scale fill the rest."""
+    blk = BLOCK[fmt]
+    if fmt == "mxfp4":
+        scales = np.ldexp(1.0, np.arange(-20, 13))
+        tops = np.array([4.0, 6.0, 7.0])
+    else:
+        scales = E4M3[1:]
+        tops = np.array([6.0])
+    borders = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0])
+    rows = []
+    for s in scales:
+        for top in tops:
+            base = torch.from_numpy(np.concatenate([[top * s], borders * s])).to(dtype)
+            bits = base.view(torch.int16).int()
+            for step in (-1, 0, 1):
+                moved = bits.clone()
+                moved[1:] += step
+                row = torch.zeros(blk, dtype=dtype)
+                row[:8] = moved.to(torch.int16).view(dtype)
+                rows.append(row)
+    x = torch.stack(rows).cuda()
+    x = torch.cat([x, -x])
+    q, qt = g.quantize_mx_both(x, fmt)
+    check_quantised(q, to64(x), fmt)
+    check_quantised(qt, to64(x).T, fmt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("offset", range(8))
+def test_quantise_rows_at_every_offset(offset, dtype, fmt):
+    """Rows that start anywhere between two 16-byte boundaries, odd row distances, tiles cut at either end; what lies
+    around the matrix is NaN and stays where it is."""
+    for rows, cols, ld in ((130, 259, 301), (3, 1, 9), (129, 127, 128), (40, 131, 137), (2, 300, 300)):
+        pool = torch.full((offset + rows * ld + 16,), math.nan, dtype=dtype, device="cuda")
+        x = pool[offset:offset + rows * ld].view(rows, ld)[:, :cols]
+        x.copy_(activations(rows, cols, dtype, rows + offset).cuda())
+        q, qt = g.quantize_mx_both(x, fmt)
+        values = check_quantised(q, to64(x), fmt)
+        check_quantised(qt, to64(x).T, fmt)
+        one = g.quantize_mx(x, fmt)
+        assert torch.equal(one.data, q.data) and torch.equal(one.scales, q.scales)
+        back = pool.clone()
+        g.dequantize_mx(q, out=back[offset:offset + rows * ld].view(rows, ld)[:, :cols])
+        inside = torch.zeros_like(pool, dtype=torch.bool)
+        inside[offset:offset + rows * ld].view(rows, ld)[:, :cols] = True
+        assert back[~inside].isnan().all()
+        np.testing.assert_array_equal(to64(back[inside]), to64(torch.from_numpy(values).float().to(dtype)).reshape(-1))
