@@ -70,55 +70,54 @@ __device__ __forceinline__ void read_shifted(uint32_t (&w)[4], const uint8_t* ro
   for (int k = 0; k < 4; ++k) w[k] = (at & 1) ? __funnelshift_r(v[k], v[k + 1], 16) : v[k];
 }
 
-// The block's scale byte and what its elements are multiplied with; `amax` = largest magnitude as bits.
-// clip > 0 asks for the elements to be clipped to it first (the product would leave fp32's range).
+// The scale byte of a block whose largest magnitude is `amax` (as bits), and its factor: what the elements are
+// multiplied with; negative where they are first to be clipped to 2688 t (their product would leave
+// fp32's range), NaN for a block that holds a NaN or an infinity.
 template <int FMT, int F16>
-__device__ __forceinline__ void block_scale(uint32_t amax, float inv_t, uint32_t* byte, float* mult, bool* bad,
-                                            bool* saturated) {
-  *bad = amax >= (F16 ? 0x7C00u : 0x7F80u);
-  *saturated = false;
+__device__ __forceinline__ float block_scale(uint32_t amax, float inv_t, uint32_t* byte) {
+  const bool bad = amax >= (F16 ? 0x7C00u : 0x7F80u);
   const float a = half_bits_to_float<F16>(amax);
+  float factor;
   if constexpr (FMT == kMxfp4) {
     const int e = static_cast<int>(__float_as_uint(a) >> 23) - 2;  // biased exponent of the scale
     const uint32_t b = static_cast<uint32_t>(e > 0 ? e : 0);
-    *byte = *bad ? 255u : b;
-    *mult = __uint_as_float((254u - b) << 23);
+    *byte = bad ? 255u : b;
+    factor = __uint_as_float((254u - b) << 23);
   } else {
     const float scaled = a * inv_t;
-    *saturated = scaled > 2688.0f;
     const float sixth = fminf(scaled, 2688.0f) * (1.0f / 6.0f);
     const float c = sixth * 4097.0f;
     const uint32_t b = e4m3_byte(__fsub_rn(c, __fsub_rn(c, sixth)));
-    *byte = *bad ? 127u : b;
+    *byte = bad ? 127u : b;
     float r;
     asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(e4m3_value(b)));
-    *mult = b == 0u ? 0.0f : r;
+    factor = b == 0u ? 0.0f : scaled > 2688.0f ? -r : r * inv_t;
   }
+  return bad ? __uint_as_float(0x7FC00000u) : factor;
 }
 
 // Eight elements (two to a word) -> eight codes.
 template <int FMT, int F16>
-__device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], float inv_t, float mult, bool bad, bool saturated) {
+__device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], float inv_t, float factor) {
   float v[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     v[j] = half_bits_to_float<F16>((j & 1) ? w[j / 2] >> 16 : w[j / 2] & 0xFFFFu);
   }
   if constexpr (FMT == kNvfp4) {
-    if (saturated) {
+    if (factor < 0.0f) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j] * inv_t, -2688.0f), 2688.0f);
     }
-    const float m = saturated ? mult : mult * inv_t;
     constexpr float kRound = 768.0f;  // numbers from 512 to 1024 are multiples of 2^-14
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __fsub_rn(__fmaf_rn(v[j], m, kRound), kRound);
+    for (int j = 0; j < 8; ++j) v[j] = __fsub_rn(__fmaf_rn(v[j], fabsf(factor), kRound), kRound);
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= mult;
+    for (int j = 0; j < 8; ++j) v[j] *= factor;
   }
   const uint32_t codes = e2m1_pack8(v);
-  return bad ? 0u : codes;
+  return factor == factor ? codes : 0u;
 }
 
 // ROW / COL: which forms are written. VEC: rows of x start on 16 bytes.
@@ -206,27 +205,38 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_co
     }
   }
   if constexpr (ROW) {
+    constexpr int kLanes = mx_block(FMT) / 8;  // lanes that share a block
+    // Two passes at a time: the lanes of an NVFP4 block each work out the scale of one of them (the scale costs as
+    // much as eight elements) and exchange the factors.
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      const int r = p * 16 + (t >> 4);
-      uint32_t m = __vmaxu2(__vmaxu2(w[p][0] & 0x7FFF7FFFu, w[p][1] & 0x7FFF7FFFu),
-                            __vmaxu2(w[p][2] & 0x7FFF7FFFu, w[p][3] & 0x7FFF7FFFu));
-      m = max(m & 0xFFFFu, m >> 16);
-      m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-      if constexpr (FMT == kMxfp4) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-      uint32_t byte;
-      float mult;
-      bool bad, sat;
-      block_scale<FMT, F16>(m, args.inv_t, &byte, &mult, &bad, &sat);
-      const uint32_t codes = quantise8<FMT, F16>(w[p], args.inv_t, mult, bad, sat);
-      const long long row = r0 + r;
-      if (row < args.rows && col / 2 + 4 <= args.pitch[0]) {
-        *reinterpret_cast<uint32_t*>(args.data[0] + row * args.pitch[0] + col / 2) = codes;
+    for (int p = 0; p < 8; p += 2) {
+      uint32_t m[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t(&v)[4] = w[p + h];
+        m[h] = __vmaxu2(__vmaxu2(v[0] & 0x7FFF7FFFu, v[1] & 0x7FFF7FFFu), __vmaxu2(v[2] & 0x7FFF7FFFu, v[3] & 0x7FFF7FFFu));
+        m[h] = max(m[h] & 0xFFFFu, m[h] >> 16);
+        m[h] = max(m[h], __shfl_xor_sync(0xFFFFFFFFu, m[h], 1));
+        if constexpr (FMT == kMxfp4) m[h] = max(m[h], __shfl_xor_sync(0xFFFFFFFFu, m[h], 2));
       }
-      constexpr int kLanes = mx_block(FMT) / 8;  // lanes that share a block
-      if (piece % kLanes == 0) {
-        const int block = piece / kLanes;
+      float factor[2];
+      uint32_t byte;
+      const int own = piece & 1;  // the pass whose scale this lane works out
+      const float mine = block_scale<FMT, F16>(own ? m[1] : m[0], args.inv_t, &byte);
+      const float other = __shfl_xor_sync(0xFFFFFFFFu, mine, 1);
+      factor[0] = own ? other : mine;
+      factor[1] = own ? mine : other;
+      if (piece % kLanes < 2) {
+        const int block = piece / kLanes, r = (p + own) * 16 + (t >> 4);
         scale_row[(block / 4) * kMxGroupBytes + (r % 32) * 16 + (r / 32) * 4 + block % 4] = static_cast<uint8_t>(byte);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t codes = quantise8<FMT, F16>(w[p + h], args.inv_t, factor[h]);
+        const long long row = r0 + (p + h) * 16 + (t >> 4);
+        if (row < args.rows && col / 2 + 4 <= args.pitch[0]) {
+          *reinterpret_cast<uint32_t*>(args.data[0] + row * args.pitch[0] + col / 2) = codes;
+        }
       }
     }
   }
@@ -256,16 +266,14 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_co
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t byte;
-        float mult;
-        bool bad, sat;
-        block_scale<FMT, F16>(h ? m >> 16 : m & 0xFFFFu, args.inv_t, &byte, &mult, &bad, &sat);
+        const float factor = block_scale<FMT, F16>(h ? m >> 16 : m & 0xFFFFu, args.inv_t, &byte);
 #pragma unroll
         for (int g = 0; g < kBlk / 8; ++g) {
           const uint32_t* s = &v[b * kBlk + g * 8];
           const uint32_t sel = h ? 0x7632u : 0x5410u;  // the upper or lower halves of two words
           const uint32_t e[4] = {__byte_perm(s[0], s[1], sel), __byte_perm(s[2], s[3], sel),
                                  __byte_perm(s[4], s[5], sel), __byte_perm(s[6], s[7], sel)};
-          codes[h][b * (kBlk / 8) + g] = quantise8<FMT, F16>(e, args.inv_t, mult, bad, sat);
+          codes[h][b * (kBlk / 8) + g] = quantise8<FMT, F16>(e, args.inv_t, factor);
         }
         const int r = cp * 2 + h, block = rb * (32 / kBlk) + b;
         scale_col[(block / 4) * kMxGroupBytes + (r % 32) * 16 + (r / 32) * 4 + block % 4] = static_cast<uint8_t>(byte);
