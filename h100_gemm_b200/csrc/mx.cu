@@ -265,6 +265,7 @@ int b200_mx_dequantize(int format, int f16, int rows, int cols, const void* data
   if (!format_known(format) || rows <= 0 || cols <= 0 || X == nullptr || ldx < cols) return B200_ERR_INVALID_ARG;
   if (data == nullptr || scales == nullptr || !aligned16(data) || !aligned16(scales)) return B200_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(X) & 1u) != 0) return B200_ERR_INVALID_ARG;
+  if (!(tensor_scale > 0.0f) || tensor_scale > 3.4e38f || (format == B200_MXFP4 && tensor_scale != 1.0f)) return B200_ERR_INVALID_ARG;
   DequantArgs args;
   args.data = static_cast<const uint8_t*>(data);
   args.scales = static_cast<const uint8_t*>(scales);

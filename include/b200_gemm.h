@@ -289,7 +289,7 @@ size_t b200_mx_scale_bytes(int format, int rows, int cols);
 int b200_mx_quantize(int format, int f16, int rows, int cols, const void* X, long long ldx, float tensor_scale,
                      void* data, void* scales, void* data_t, void* scales_t, void* stream);
 
-/* The values: X = code * scale * tensor_scale, rounded once to bf16 or fp16. */
+/* The values: X = code * scale * tensor_scale (any positive number; 1 for MXFP4), rounded once to bf16 or fp16. */
 int b200_mx_dequantize(int format, int f16, int rows, int cols, const void* data, const void* scales,
                        float tensor_scale, void* X, long long ldx, void* stream);
 

@@ -194,7 +194,9 @@ def test_refusals_of_the_c_abi():
     for args in ((2, 0, 4, 4, 64, p, p, p, p, p), (0, 0, 0, 4, 64, p, p, p, p, p), (0, 0, 4, 4, 0, p, p, p, p, p),
                  (0, 0, 4, 4, 64, None, p, p, p, p), (0, 0, 4, 4, 64, p, p + 1, p, p, p), (0, 0, 4, 4, 64, p, p, p, p, p + 1)):
         assert lib.b200_gemm_mx(*args, 1.0, 0.0, None) == api.STATUS_INVALID_ARG, args
-    for args in ((3, 0, 4, 64, p, p, 1.0, p, 64), (0, 0, 4, 64, p + 1, p, 1.0, p, 64), (0, 0, 4, 64, p, p, 1.0, p, 63)):
+    for args in ((3, 0, 4, 64, p, p, 1.0, p, 64), (0, 0, 4, 64, p + 1, p, 1.0, p, 64), (0, 0, 4, 64, p, p, 1.0, p, 63),
+                 (0, 0, 4, 64, p, p, 2.0, p, 64), (1, 0, 4, 64, p, p, 0.0, p, 64), (1, 0, 4, 64, p, p, math.nan, p, 64),
+                 (1, 0, 4, 64, p, p, math.inf, p, 64)):
         assert lib.b200_mx_dequantize(*args, None) == api.STATUS_INVALID_ARG, args
 
 
