@@ -90,10 +90,47 @@ __device__ __forceinline__ float block_scale(uint32_t amax, float inv_t, uint32_
     const uint32_t b = e4m3_byte(__fsub_rn(c, __fsub_rn(c, sixth)));
     *byte = bad ? 127u : b;
     float r;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(e4m3_value(b)));
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(__uint_as_float(b << 20) * 1.329227995784916e36f));  // (e4m3_value)
     factor = b == 0u ? 0.0f : scaled > 2688.0f ? -r : r * inv_t;
   }
   return bad ? __uint_as_float(0x7FC00000u) : factor;
+}
+
+// Two fp32 numbers at once: the SM's packed arithmetic halves what an element costs.
+struct Pair {
+  uint64_t v;
+};
+__device__ __forceinline__ Pair pair_of(float lo, float hi) {
+  Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+  return p;
+}
+__device__ __forceinline__ Pair pair_mul(Pair a, Pair b) {
+  Pair p;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
+__device__ __forceinline__ Pair pair_fma(Pair a, Pair b, Pair c) {
+  Pair p;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return p;
+}
+__device__ __forceinline__ Pair pair_add(Pair a, Pair b) {
+  Pair p;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+  return p;
+}
+
+// The larger of the magnitudes of two pairs of 16-bit numbers (NaN wins), with signs to be ignored.
+template <int F16>
+__device__ __forceinline__ uint32_t max_magnitude2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (F16) {
+    asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  } else {
+    asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  }
+  return r;
 }
 
 // Eight elements (two to a word) -> eight codes.
@@ -109,12 +146,19 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], float inv_
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = fminf(fmaxf(v[j] * inv_t, -2688.0f), 2688.0f);
     }
-    constexpr float kRound = 768.0f;  // numbers from 512 to 1024 are multiples of 2^-14
+  }
+  const float m = FMT == kNvfp4 ? fabsf(factor) : factor;
+  const Pair mm = pair_of(m, m);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = __fsub_rn(__fmaf_rn(v[j], fabsf(factor), kRound), kRound);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= factor;
+  for (int j = 0; j < 8; j += 2) {
+    Pair p = pair_of(v[j], v[j + 1]);
+    if constexpr (FMT == kNvfp4) {
+      constexpr float kRound = 768.0f;  // numbers from 512 to 1024 are multiples of 2^-14
+      p = pair_add(pair_fma(p, mm, pair_of(kRound, kRound)), pair_of(-kRound, -kRound));
+    } else {
+      p = pair_mul(p, mm);
+    }
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(v[j]), "=f"(v[j + 1]) : "l"(p.v));
   }
   const uint32_t codes = e2m1_pack8(v);
   return factor == factor ? codes : 0u;
@@ -214,8 +258,8 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_co
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t(&v)[4] = w[p + h];
-        m[h] = __vmaxu2(__vmaxu2(v[0] & 0x7FFF7FFFu, v[1] & 0x7FFF7FFFu), __vmaxu2(v[2] & 0x7FFF7FFFu, v[3] & 0x7FFF7FFFu));
-        m[h] = max(m[h] & 0xFFFFu, m[h] >> 16);
+        m[h] = max_magnitude2<F16>(max_magnitude2<F16>(v[0], v[1]), max_magnitude2<F16>(v[2], v[3]));
+        m[h] = max(m[h] & 0x7FFFu, (m[h] >> 16) & 0x7FFFu);
         m[h] = max(m[h], __shfl_xor_sync(0xFFFFFFFFu, m[h], 1));
         if constexpr (FMT == kMxfp4) m[h] = max(m[h], __shfl_xor_sync(0xFFFFFFFFu, m[h], 2));
       }
@@ -260,13 +304,13 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_kernel(const __grid_co
     constexpr int kBlk = mx_block(FMT);
 #pragma unroll
     for (int b = 0; b < 32 / kBlk; ++b) {
-      uint32_t m = 0u;
+      uint32_t m = v[b * kBlk];
 #pragma unroll
-      for (int j = 0; j < kBlk; ++j) m = __vmaxu2(m, v[b * kBlk + j] & 0x7FFF7FFFu);
+      for (int j = 1; j < kBlk; ++j) m = max_magnitude2<F16>(m, v[b * kBlk + j]);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint32_t byte;
-        const float factor = block_scale<FMT, F16>(h ? m >> 16 : m & 0xFFFFu, args.inv_t, &byte);
+        const float factor = block_scale<FMT, F16>((h ? m >> 16 : m) & 0x7FFFu, args.inv_t, &byte);
 #pragma unroll
         for (int g = 0; g < kBlk / 8; ++g) {
           const uint32_t* s = &v[b * kBlk + g * 8];
