@@ -3,7 +3,7 @@ from __future__ import annotations
 
 from . import api
 from .api import STATUS_WORKSPACE, GemmError
-from .mx import FORMATS, MxTensor, _half_type, _invalid, _output, _require_cuda, _run
+from .mx import FORMATS, MxTensor, _current, _elsewhere, _half_type, _invalid, _output, _require_cuda
 
 MAX_TOKENS, MAX_EXPERTS, MAX_TOP_K = 64, 512, 32
 
@@ -90,18 +90,27 @@ def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: 
         w1 = (-1, pointer(w_gate_up, "w_gate_up", dtype), None, 1.0)
         w2 = (pointer(w_down, "w_down", dtype), None, 1.0)
 
-    def body(handle):
-        y = out if out is not None else torch.empty_like(x)
-        ws = workspace if workspace is not None else torch.empty(need, dtype=torch.uint8, device=device)
-        ids = weights = ids_ptr = weights_ptr = None
-        if return_routing:
-            ids = torch.empty((T, top_k), dtype=torch.int32, device=device)
-            weights = torch.empty((T, top_k), dtype=torch.float32, device=device)
-            ids_ptr, weights_ptr = ids.data_ptr(), weights.data_ptr()
-        rc = api.library().b200_moe_layer(f16, T, E, top_k, H, I, x_ptr, router_ptr, bias_ptr, *w1, *w2, 1 if renormalize else 0,
-                                          y.data_ptr(), ids_ptr, weights_ptr, ws.data_ptr(), need, handle)
-        if rc:
-            api._check(rc)
-        return (y, ids, weights) if return_routing else y
+    sizes = (f16, T, E, top_k, H, I, x_ptr, router_ptr, bias_ptr, *w1, *w2, 1 if renormalize else 0)
+    handle = _current(device, stream)
+    if handle is not False:
+        return _launch(x, sizes, need, top_k, out, return_routing, workspace, handle)
+    with _elsewhere(device, stream) as handle:
+        return _launch(x, sizes, need, top_k, out, return_routing, workspace, handle)
 
-    return _run(device, stream, body)
+
+def _launch(x, sizes, need, top_k, out, return_routing, workspace, handle):
+    import torch
+    device = x.device
+    if out is None:
+        out = torch.empty_like(x)
+    if workspace is None:
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    ids = weights = ids_ptr = weights_ptr = None
+    if return_routing:
+        ids = torch.empty(x.shape[0], top_k, dtype=torch.int32, device=device)
+        weights = torch.empty(x.shape[0], top_k, dtype=torch.float32, device=device)
+        ids_ptr, weights_ptr = ids.data_ptr(), weights.data_ptr()
+    rc = api.library().b200_moe_layer(*sizes, out.data_ptr(), ids_ptr, weights_ptr, workspace.data_ptr(), need, handle)
+    if rc:
+        api._check(rc)
+    return (out, ids, weights) if return_routing else out

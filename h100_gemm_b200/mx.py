@@ -160,13 +160,12 @@ def _elsewhere(device, stream):
             yield handle or None
 
 
-def _run(device, stream, body):
-    """body(stream handle) on the tensors' device and stream; the usual case, the current ones, costs two lookups."""
+def _current(device, stream):
+    """The current stream's handle where a call can run as it is, the usual case; else False (see _elsewhere)."""
     import torch
     if stream is None and torch.cuda.current_device() == device.index:
-        return body(torch._C._cuda_getCurrentRawStream(device.index) or None)
-    with _elsewhere(device, stream) as handle:
-        return body(handle)
+        return torch._C._cuda_getCurrentRawStream(device.index) or None
+    return False
 
 
 def _require_cuda(device, name: str, expected=None):
@@ -203,29 +202,36 @@ def _quantize(x, format, tensor_scale, out, rows: bool, cols: bool, stream):
     f16 = _half_type(x.dtype, "x")
     if x.dim() != 2 or x.numel() == 0:
         raise _invalid("x must be a 2-D tensor with at least one row and one column")
-    R, C = x.shape
     ld = _row_stride(x, "x")
     device = x.device
     _require_cuda(device, "x")
     if format == "mxfp4" and tensor_scale != 1.0:
         raise _invalid("mxfp4 has no tensor scale (it must be 1)")
     if out is not None:
-        want = (R, C) if rows else (C, R)
+        want = tuple(x.shape) if rows else tuple(x.shape)[::-1]
         if (out.rows, out.cols) != want or out.format != format or out.tensor_scale != tensor_scale:
             raise _invalid(f"out must be a [{want[0]}, {want[1]}] {format} matrix with tensor scale {tensor_scale}")
         _require_cuda(out.device, "out", device)
+    handle = _current(device, stream)
+    if handle is not False:
+        return _launch_quantize(x, fmt, f16, ld, format, tensor_scale, out, rows, cols, handle)
+    with _elsewhere(device, stream) as handle:
+        return _launch_quantize(x, fmt, f16, ld, format, tensor_scale, out, rows, cols, handle)
 
-    def body(handle):
-        q = (out or MxTensor._empty(R, C, format, tensor_scale, device)) if rows else None
-        qt = (out or MxTensor._empty(C, R, format, tensor_scale, device)) if cols else None
-        rc = api.library().b200_mx_quantize(
-            fmt, f16, R, C, x.data_ptr(), ld, tensor_scale, q._data_ptr if rows else None, q._scales_ptr if rows else None,
-            qt._data_ptr if cols else None, qt._scales_ptr if cols else None, handle)
-        if rc:
-            api._check(rc)
-        return q, qt
 
-    return _run(device, stream, body)
+def _launch_quantize(x, fmt, f16, ld, format, tensor_scale, out, rows, cols, handle):
+    R, C = x.shape
+    q = qt = data = scales = data_t = scales_t = None
+    if rows:
+        q = out or MxTensor._empty(R, C, format, tensor_scale, x.device)
+        data, scales = q._data_ptr, q._scales_ptr
+    if cols:
+        qt = out or MxTensor._empty(C, R, format, tensor_scale, x.device)
+        data_t, scales_t = qt._data_ptr, qt._scales_ptr
+    rc = api.library().b200_mx_quantize(fmt, f16, R, C, x.data_ptr(), ld, tensor_scale, data, scales, data_t, scales_t, handle)
+    if rc:
+        api._check(rc)
+    return q, qt
 
 
 def quantize_mx(x, format: str = "mxfp4", transpose: bool = False, tensor_scale: float = 1.0, out=None,
@@ -254,21 +260,28 @@ def dequantize_mx(q: MxTensor, dtype=None, out=None, stream=None):
     import torch
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
     f16 = _half_type(dtype, "dtype")
-    device, shape = q.device, (q.rows, q.cols)
+    device = q.device
     _require_cuda(device, "q")
     if out is not None:
-        _output(out, shape, dtype, device, False)
+        _output(out, (q.rows, q.cols), dtype, device, False)
 
-    def body(handle):
-        y = out if out is not None else torch.empty(shape, dtype=dtype, device=device)
-        rc = api.library().b200_mx_dequantize(FORMATS[q.format], f16, q.rows, q.cols, q._data_ptr, q._scales_ptr,
-                                              q.tensor_scale, y.data_ptr(), q.cols if out is None else _row_stride(out, "out"),
-                                              handle)
-        if rc:
-            api._check(rc)
-        return y
+    ld = q.cols if out is None else _row_stride(out, "out")
+    handle = _current(device, stream)
+    if handle is not False:
+        return _launch_dequantize(q, dtype, f16, out, ld, handle)
+    with _elsewhere(device, stream) as handle:
+        return _launch_dequantize(q, dtype, f16, out, ld, handle)
 
-    return _run(device, stream, body)
+
+def _launch_dequantize(q, dtype, f16, out, ld, handle):
+    import torch
+    if out is None:
+        out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
+    rc = api.library().b200_mx_dequantize(FORMATS[q.format], f16, q.rows, q.cols, q._data_ptr, q._scales_ptr, q.tensor_scale,
+                                          out.data_ptr(), ld, handle)
+    if rc:
+        api._check(rc)
+    return out
 
 
 def gemm_mx(a: MxTensor, b: MxTensor, out=None, alpha: float = 1.0, beta: float = 0.0, dtype=None, stream=None):
@@ -281,18 +294,25 @@ def gemm_mx(a: MxTensor, b: MxTensor, out=None, alpha: float = 1.0, beta: float 
         raise _invalid(f"a is {a.format}, b is {b.format}")
     if a.cols != b.cols:
         raise _invalid("a and b disagree on K")
-    device, shape = a.device, (a.rows, b.rows)
+    device = a.device
     _require_cuda(device, "a")
     _require_cuda(b.device, "b", device)
     if out is not None:
-        _output(out, shape, dtype, device, True)
+        _output(out, (a.rows, b.rows), dtype, device, True)
 
-    def body(handle):
-        c = out if out is not None else torch.empty(shape, dtype=dtype, device=device)
-        rc = api.library().b200_gemm_mx(FORMATS[a.format], f16, a.rows, b.rows, a.cols, a._data_ptr, a._scales_ptr, b._data_ptr,
-                                        b._scales_ptr, c.data_ptr(), alpha * a.tensor_scale * b.tensor_scale, beta, handle)
-        if rc:
-            api._check(rc)
-        return c
+    handle = _current(device, stream)
+    if handle is not False:
+        return _launch_gemm(a, b, dtype, f16, out, alpha, beta, handle)
+    with _elsewhere(device, stream) as handle:
+        return _launch_gemm(a, b, dtype, f16, out, alpha, beta, handle)
 
-    return _run(device, stream, body)
+
+def _launch_gemm(a, b, dtype, f16, out, alpha, beta, handle):
+    import torch
+    if out is None:
+        out = torch.empty(a.rows, b.rows, dtype=dtype, device=a.device)
+    rc = api.library().b200_gemm_mx(FORMATS[a.format], f16, a.rows, b.rows, a.cols, a._data_ptr, a._scales_ptr, b._data_ptr,
+                                    b._scales_ptr, out.data_ptr(), alpha * a.tensor_scale * b.tensor_scale, beta, handle)
+    if rc:
+        api._check(rc)
+    return out
