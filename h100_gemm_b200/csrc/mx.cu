@@ -294,6 +294,7 @@ int b200_mx_dequantize(int format, int f16, int rows, int cols, const void* data
 int b200_gemm_mx(int format, int f16, int M, int N, int K, const void* A, const void* A_scales, const void* B,
                  const void* B_scales, void* C, float alpha, float beta, void* stream) {
   if (!format_known(format) || M <= 0 || N <= 0 || K <= 0) return B200_ERR_INVALID_ARG;
+  if (M > 0x7FFFFFFF - 512 || N > 0x7FFFFFFF - 512 || K > 0x7FFFFFFF - 512) return B200_ERR_INVALID_ARG;  // (tiles end in 32 bits)
   if (A == nullptr || A_scales == nullptr || B == nullptr || B_scales == nullptr || C == nullptr) return B200_ERR_INVALID_ARG;
   if (!aligned16(A) || !aligned16(A_scales) || !aligned16(B) || !aligned16(B_scales)) return B200_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(C) & 1u) != 0) return B200_ERR_INVALID_ARG;

@@ -17,7 +17,6 @@ blocks have to run along the contraction::
 from __future__ import annotations
 
 import contextlib
-import math
 
 from . import api
 from .api import STATUS_INVALID_ARG, GemmError
@@ -60,8 +59,8 @@ class MxTensor:
         _format(format)
         if rows <= 0 or cols <= 0:
             raise _invalid("rows and cols must be positive")
-        if not (tensor_scale > 0 and math.isfinite(tensor_scale)):
-            raise _invalid("tensor_scale must be positive and finite")
+        if not 0 < tensor_scale < 3.4e38:
+            raise _invalid("tensor_scale must be positive and finite in fp32")
         if format == "mxfp4" and tensor_scale != 1.0:
             raise _invalid("mxfp4 has no tensor scale (it must be 1)")
         pointers = []
@@ -258,6 +257,8 @@ def _output(out, shape, dtype, device, contiguous: bool) -> None:
 def dequantize_mx(q: MxTensor, dtype=None, out=None, stream=None):
     """The values of q as a [rows, cols] bf16 (default) or fp16 tensor."""
     import torch
+    if not isinstance(q, MxTensor):
+        raise _invalid(f"q must be an MxTensor, got {type(q).__name__}")
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
     f16 = _half_type(dtype, "dtype")
     device = q.device
@@ -288,6 +289,8 @@ def gemm_mx(a: MxTensor, b: MxTensor, out=None, alpha: float = 1.0, beta: float 
     """out[M, N] = (a[M, K] @ b[N, K]^T) * alpha + beta for two 4-bit matrices of one format, tensor scales
     applied; bf16 (default) or fp16 output, fp32 accumulation."""
     import torch
+    if not isinstance(a, MxTensor) or not isinstance(b, MxTensor):
+        raise _invalid(f"a and b must be MxTensors, got {type(a).__name__} and {type(b).__name__}")
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
     f16 = _half_type(dtype, "dtype")
     if a.format != b.format:

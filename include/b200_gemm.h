@@ -272,7 +272,8 @@ int b200_reference_gpu_gemm_f16(int M, int N, int K, const void* A, const void* 
  *         of 512 bytes, each the scales of 4 consecutive blocks of all 128 rows, with row r's
  *         block b at byte (r % 32) * 16 + (r / 32) * 4 + b % 4. Rows and columns are padded to whole tiles;
  *         the padding's bytes are zero (a padding byte that stands for NaN would spoil results).
- * Both start on 16 bytes. The two sizes: */
+ * Both start on 16 bytes. The first call of any of these operators on a device does the library's one-time set-up:
+ * make it outside stream capture. The two sizes: */
 typedef enum b200_mx_format { B200_MXFP4 = 0, B200_NVFP4 = 1 } b200_mx_format;
 size_t b200_mx_data_bytes(int rows, int cols);
 size_t b200_mx_scale_bytes(int format, int rows, int cols);

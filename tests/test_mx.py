@@ -169,6 +169,9 @@ def test_refusals_without_a_device():
         cpu_mx(4, 64, "mxfp4", 2.0)
     with pytest.raises(g.GemmError):
         cpu_mx(4, 64, "nvfp4", math.inf)
+    for call in (lambda: g.gemm_mx(x, cpu_mx(4, 64)), lambda: g.gemm_mx(cpu_mx(4, 64), x), lambda: g.dequantize_mx(x)):
+        with pytest.raises(g.GemmError, match="MxTensor"):
+            call()
     good = cpu_mx(4, 64)
     with pytest.raises(g.GemmError, match="bytes"):
         g.MxTensor(good.data, good.scales, 5, 64)
@@ -192,7 +195,7 @@ def test_refusals_of_the_c_abi():
                dict(fmt=1, ts=0.0), dict(fmt=1, ts=-1.0), dict(fmt=1, ts=math.nan), dict(fmt=1, ts=2.0 ** 65)):
         assert quant(**kw) == api.STATUS_INVALID_ARG, kw
     for args in ((2, 0, 4, 4, 64, p, p, p, p, p), (0, 0, 0, 4, 64, p, p, p, p, p), (0, 0, 4, 4, 0, p, p, p, p, p),
-                 (0, 0, 4, 4, 64, None, p, p, p, p), (0, 0, 4, 4, 64, p, p + 1, p, p, p), (0, 0, 4, 4, 64, p, p, p, p, p + 1)):
+                 (0, 0, 4, 4, 64, None, p, p, p, p), (0, 0, 4, 4, 64, p, p + 1, p, p, p), (0, 0, 4, 4, 64, p, p, p, p, p + 1), (0, 0, 2 ** 31 - 1, 4, 64, p, p, p, p, p)):
         assert lib.b200_gemm_mx(*args, 1.0, 0.0, None) == api.STATUS_INVALID_ARG, args
     for args in ((3, 0, 4, 64, p, p, 1.0, p, 64), (0, 0, 4, 64, p + 1, p, 1.0, p, 64), (0, 0, 4, 64, p, p, 1.0, p, 63),
                  (0, 0, 4, 64, p, p, 2.0, p, 64), (1, 0, 4, 64, p, p, 0.0, p, 64), (1, 0, 4, 64, p, p, math.nan, p, 64),
@@ -530,3 +533,52 @@ def test_quantise_rows_at_every_offset(offset, dtype, fmt):
         inside[offset:offset + rows * ld].view(rows, ld)[:, :cols] = True
         assert back[~inside].isnan().all()
         np.testing.assert_array_equal(to64(back[inside]), to64(torch.from_numpy(values).float().to(dtype)).reshape(-1))
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Passes on two streams without any wait between them: nothing is shared."""
+    gen = torch.Generator().manual_seed(6)
+    xs = [torch.randn(m, 2048, generator=gen).bfloat16().cuda() for m in (8, 100, 300, 700)]
+    ws = [g.quantize_mx((torch.randn(n, 2048, generator=gen) * 0.02).bfloat16().cuda(), "mxfp4") for n in (640, 1000)]
+    want = [[g.gemm_mx(g.quantize_mx(x), w) for x in xs] for w in ws]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in ws]
+    got = [[], []]
+    for _ in range(4):
+        for x in xs:
+            for i, (s, w) in enumerate(zip(streams, ws)):
+                got[i].append(g.gemm_mx(g.quantize_mx(x, stream=s), w, stream=s))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for j, out in enumerate(got[i]):
+            assert torch.equal(out, want[i][j % len(xs)])
+    assert g.device_status()[0] == api.STATUS_OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_offsets_beyond_32_bits(fmt):
+    """A matrix of more than 2^32 elements: its first and last rows both ways, read back, and multiplied."""
+    R, C = 131077, 32808
+    x = torch.empty(R, C, dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for r in range(0, R, 16384):
+        x[r:r + 16384] = torch.randn(min(16384, R - r), C, generator=gen, device="cuda")
+    q, qt = g.quantize_mx_both(x, fmt)
+    rows = [0, 1, 65535, 65536, R - 130, R - 1]
+    value = quantise_ref(to64(x[rows]), fmt)[2]
+    back = g.dequantize_mx(q)
+    np.testing.assert_array_equal(to64(back[rows]), value)
+    cols = [0, 5, 16384, C - 1]
+    value_t = quantise_ref(to64(x[:, cols]).T.copy(), fmt)[2]
+    back = g.dequantize_mx(qt)
+    np.testing.assert_array_equal(to64(back[cols]), value_t)
+    del back, x
+    a = g.quantize_mx(torch.randn(3, C, generator=gen, device="cuda").bfloat16(), fmt)
+    av = to64(g.dequantize_mx(a))
+    out = g.gemm_mx(a, q)
+    ref = av @ value.T
+    assert (np.abs(to64(out[:, rows]) - ref) <= product_bound(av, value, ref, torch.bfloat16)).all()
+    out = g.gemm_mx(q, a)  # the long side as rows of C
+    assert (np.abs(to64(out[rows]) - ref.T) <= product_bound(value, av, ref.T, torch.bfloat16)).all()
