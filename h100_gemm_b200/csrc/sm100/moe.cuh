@@ -733,11 +733,12 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __gri
   float4* red = reinterpret_cast<float4*>(smem);  // two buffers, used in turn
   const int stride = gate_up_stride(MoeUnit<W>::kTiles, args.T);
   const RouteTables r = route_tables_at(smem + 2 * kMoeWarps * stride * 16, args);
-  ptx::grid_launch_dependents();
   const int strips = (args.I + kCols - 1) / kCols;
   const int by_index = static_cast<int>(gridDim.x) / strips, by_strip = static_cast<int>(gridDim.x) % strips;
   UnitCursor unit{static_cast<int>(blockIdx.x) / strips, static_cast<int>(blockIdx.x) % strips};
   ptx::grid_dependency_wait();
+  // Only now: a CTA of the down kernel then starts knowing that the router has completed.
+  ptx::grid_launch_dependents();
   build_route_tables(r, args);
   GateUp<W, F16> g{args, r, ptx::lane_id(), static_cast<int>(threadIdx.x) / 32, *r.count, {}};
   if (unit.index < g.experts && g.warp * kMoeStep < args.H) g.load(unit, g.warp * kMoeStep);
@@ -825,12 +826,15 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_c
   const int rank = split > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
   D d{args, r, ptx::lane_id(), static_cast<int>(blockIdx.x) / split * 16 * D::MT, (args.I + kMoeStep - 1) / kMoeStep, {}};
   for (int i = static_cast<int>(threadIdx.x); i < kMoeWarps * per_warp; i += kMoeThreads) sums[i] = 0.0f;
-  ptx::grid_launch_dependents();
-  ptx::grid_dependency_wait();
+  // The routing and the weights are there already: every CTA of the gate/up kernel had waited for the router before this
+  // kernel was allowed to start. So the first step's weights are under way while that kernel finishes; its
+  // hidden values are what the wait is for.
   build_route_tables(r, args);
   const int total = *r.count * d.steps, stride = split * kMoeWarps;
   int s = rank * kMoeWarps + warp;
   if (s < total) d.load(s);
+  ptx::grid_launch_dependents();
+  ptx::grid_dependency_wait();
   float* mine = sums + warp * per_warp;
   for (; s < total; s += stride) d.run(mine, s, s + stride, total);
   __syncthreads();
