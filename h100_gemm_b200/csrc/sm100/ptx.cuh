@@ -30,6 +30,20 @@ B200_DEVICE uint32_t lane_id() {
   return r;
 }
 
+// One lane of a converged warp. The rest of the code around an issue stays uniform for the warp, so that
+// descriptors and addresses can live in uniform registers.
+B200_DEVICE bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "}"
+      : "=r"(r));
+  return r != 0;
+}
+
 B200_DEVICE uint32_t cluster_ctarank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
