@@ -13,7 +13,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 size_t round_up(size_t x) { return (x + 255) / 256 * 256; }
 
 // Workspace: [h][ids][weights]
-size_t h_bytes(int T, int k, int I) { return round_up(static_cast<size_t>(T) * k * I * 2); }
+size_t h_bytes(int T, int k, int I) { return round_up(static_cast<size_t>(T) * k * I * 4); }
 size_t pair_bytes(int T, int k) { return round_up(static_cast<size_t>(T) * k * 4); }
 
 bool sizes_ok(int T, int E, int k, int H, int I) {

@@ -3,11 +3,13 @@
 //   logits  l[t, e] = x[t] . R[e] + b[e]                                        (fp32)
 //   chosen  S[t] = the k largest logits of t (ties: the lower index; -inf is never chosen)
 //   weight  p[t, e] = exp(l[t, e]) / sum of exp(l) over S[t], or over all experts
-//   gated   h[t, e] = p[t, e] * silu(G_e x[t]) * (U_e x[t])                     (fp32, rounded to 16 bits once)
+//   gated   h[t, e] = p[t, e] * silu(G_e x[t]) * (U_e x[t])                     (fp32, kept in two 16-bit parts)
 //   out[t] = sum over e in S[t] of D_e h[t, e]                                  (fp32, rounded once)
 //
-// (The routing weight goes into h before its one rounding, so the down product of all experts of a token is
-// a single sum in the accumulators.)
+// (The routing weight goes into h, so the down product of all experts of a token is a single sum. h is kept as
+// its nearest 16-bit number and the nearest 16-bit number of what that leaves, 16 bits of bf16 or 22 of fp16: one
+// part alone costs the result a second rounding, an error 1.4 times as large. The two parts ride side by side on
+// columns of the MMA that a decode step leaves empty anyway.)
 //
 // Bound by memory: every chosen expert's 3 H I weights are read once and used for a handful of
 // tokens. So the weights go straight from global memory to registers in the shape of an MMA's A
@@ -60,7 +62,7 @@ struct MoeArgs {
   float lift1, lift2;       // what sums of products with w1 / w2 are multiplied with (1 for 16-bit weights)
   int* ids;                 // [T, k], -1 = none
   float* weights;           // [T, k]
-  uint16_t* h;              // [T, k, I]
+  uint16_t* h;              // [T, k, 2, I]
   uint16_t* out;            // [T, H]
 };
 
@@ -85,6 +87,15 @@ B200_DEVICE float2 unpack16(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2*>(&w));
   } else {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+  }
+}
+
+template <int F16>
+B200_DEVICE float widen16(uint16_t bits) {
+  if constexpr (F16) {
+    return __half2float(__ushort_as_half(bits));
+  } else {
+    return __uint_as_float(static_cast<uint32_t>(bits) << 16);
   }
 }
 
@@ -716,8 +727,11 @@ struct GateUp {
         gate += at[p * stride * 4];
         up += at[p * stride * 4 + 2];
       }
-      args.h[static_cast<long long>(r.pairs[first_pair + c]) * args.I + row] =
-          round16<F16>(r.weights[first_pair + c] * (silu(gate * args.lift1) * (up * args.lift1)));
+      const float h = r.weights[first_pair + c] * (silu(gate * args.lift1) * (up * args.lift1));
+      uint16_t* to = args.h + static_cast<long long>(r.pairs[first_pair + c]) * 2 * args.I + row;
+      const uint16_t nearest = round16<F16>(h);
+      to[0] = nearest;
+      to[args.I] = round16<F16>(h - widen16<F16>(nearest));  // (NaN where h is infinite: the sum is not finite either way)
     }
   }
 };
@@ -782,23 +796,22 @@ struct Down {
     const uint16_t* b[NT];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      const int c = min((j0 + j) * 8 + static_cast<int>(lane >> 2), tokens - 1);
-      b[j] = args.h + static_cast<long long>(r.pairs[first_pair + c]) * args.I;
+      // columns 2 c and 2 c + 1 of a tile are the two parts of its token c
+      const int column = static_cast<int>(lane >> 2);
+      const int c = min((j0 + j) * 4 + column / 2, tokens - 1);
+      b[j] = args.h + (static_cast<long long>(r.pairs[first_pair + c]) * 2 + column % 2) * args.I;
     }
     float acc[NT][MT][4] = {};
     MoeStep<W, F16, NT>::mma(w, acc, b, k0, args.I, lane);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
+      const int c = (j0 + j) * 4 + static_cast<int>(lane & 3u);
+      if (c < tokens) {
+        float* to = sums + r.tokens[first_pair + c] * kPitch + (lane >> 2);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int c = (j0 + j) * 8 + static_cast<int>(lane & 3u) * 2 + n;
-        if (c < tokens) {
-          float* to = sums + r.tokens[first_pair + c] * kPitch + (lane >> 2);
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            to[m * 16] += acc[j][m][n];
-            to[m * 16 + 8] += acc[j][m][2 + n];
-          }
+        for (int m = 0; m < MT; ++m) {
+          to[m * 16] += acc[j][m][0] + acc[j][m][1];
+          to[m * 16 + 8] += acc[j][m][2] + acc[j][m][3];
         }
       }
     }
@@ -806,7 +819,7 @@ struct Down {
 
   B200_DEVICE void run(float* sums, int s, int next, int total) {
     const int tokens = r.size[s / steps], first_pair = r.first[s / steps];
-    const int n_tiles = (tokens + 7) / 8, k0 = s % steps * kMoeStep;
+    const int n_tiles = (tokens + 3) / 4, k0 = s % steps * kMoeStep;
     int j = 0;
     for (; j + 1 < n_tiles; j += 2) tiles<2>(sums, first_pair, tokens, j, k0);
     if (j < n_tiles) tiles<1>(sums, first_pair, tokens, j, k0);

@@ -54,10 +54,11 @@ def layer_ref(x, ids, weights, w1, w2):
 
 
 def allowed(dtype, out, size, up_err, I, top_k):
-    """|kernel - formula|: the output's rounding, h's rounding to 16 bits, 2^-20 for its fp32 factors (weight, sigmoid,
-    products), fp32 sums of the down product, and what gate and up bring along. fp16's h may be subnormal: 2^-25 each."""
+    """|kernel - formula|: the output's rounding, h's rounding to two 16-bit parts (the square of one's), 2^-20 for its fp32
+    factors (weight, sigmoid, products), fp32 sums of the down product, and what gate and up bring along. fp16's
+    parts may be subnormal: 2^-25 each."""
     eps = torch.finfo(dtype).eps / 2
-    return eps * out.abs() + (eps + 2.0 ** -20 + (top_k * I / 16 + 80) * 2.0 ** -22) * size + up_err + 1e-6 * (dtype == FP16) + 1e-30
+    return eps * out.abs() + (eps ** 2 + 2.0 ** -20 + (2 * top_k * I / 16 + 80) * 2.0 ** -22) * size + up_err + 1e-6 * (dtype == FP16) + 1e-30
 
 
 def make(T, E, H, I, dtype, seed, fmt=None):
@@ -97,8 +98,8 @@ def check(x, router, w1, w2, v1, v2, k, bias=None, renormalize=True, ids_known=T
 # --------------------------------------------------------------------------------------- no GPU
 def test_workspace_and_refusals_without_a_device():
     lib = api.library()
-    assert g.moe_workspace_bytes(1, 8, 2, 64, 64) == 256 + 2 * 256
-    assert g.moe_workspace_bytes(64, 128, 8, 2048, 768) == 64 * 8 * 768 * 2 + 2 * 64 * 8 * 4
+    assert g.moe_workspace_bytes(1, 8, 2, 64, 64) == 512 + 2 * 256
+    assert g.moe_workspace_bytes(64, 128, 8, 2048, 768) == 64 * 8 * 768 * 4 + 2 * 64 * 8 * 4
     for bad in ((0, 8, 2, 64, 64), (65, 8, 2, 64, 64), (1, 513, 2, 64, 64), (1, 8, 9, 64, 64), (1, 64, 33, 64, 64),
                 (1, 8, 0, 64, 64), (1, 8, 2, 60, 64), (1, 8, 2, 64, 0)):
         assert g.moe_workspace_bytes(*bad) == 0
