@@ -65,7 +65,7 @@ int launch_all(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) 
   const int most = args.T * args.k < args.E ? args.T * args.k : args.E;  // experts that can be chosen
   const long long units = static_cast<long long>(most) * ((args.I + 8 * MT - 1) / (8 * MT));
   Launch up(static_cast<int>(units < 2ll * dev.sm_count ? units : 2ll * dev.sm_count), kMoeThreads,
-            2 * kMoeWarps * gate_up_stride(MT, args.T) * 16 + tables, stream, 1);
+            gate_up_buffers(MT, args.T) * kMoeWarps * gate_up_stride(MT, args.T) * 16 + tables, stream, 1);
   B200_TRY_CUDA(cudaLaunchKernelEx(&up.config, &moe_gate_up_kernel<W, F16>, args));
 
   // Clusters share the columns of a unit until every SM has two CTAs, but no warp is left without a step.

@@ -739,14 +739,20 @@ struct GateUp {
 __host__ __device__ __forceinline__ int moe_token_tiles(int T) { return (T + 7) / 8; }
 // float4 between two warps' sums
 __host__ __device__ __forceinline__ int gate_up_stride(int tiles, int T) { return tiles * moe_token_tiles(T) * 32; }
+// Sums of two units, used in turn, save a barrier per unit; of one where two CTAs per SM have no room for more (4-bit
+// weights and 33 or more tokens: a second buffer left one CTA per SM, 167 against 141 us for 64 tokens of 128 MXFP4 experts).
+__host__ __device__ __forceinline__ int gate_up_buffers(int tiles, int T) {
+  return 2 * kMoeWarps * gate_up_stride(tiles, T) * 16 <= 80 * 1024 ? 2 : 1;
+}
 
 template <int W, int F16>
 __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __grid_constant__ MoeArgs args) {
   constexpr int kCols = GateUp<W, F16>::kCols;
   extern __shared__ __align__(16) uint8_t smem[];
-  float4* red = reinterpret_cast<float4*>(smem);  // two buffers, used in turn
+  float4* red = reinterpret_cast<float4*>(smem);
   const int stride = gate_up_stride(MoeUnit<W>::kTiles, args.T);
-  const RouteTables r = route_tables_at(smem + 2 * kMoeWarps * stride * 16, args);
+  const int buffers = gate_up_buffers(MoeUnit<W>::kTiles, args.T);
+  const RouteTables r = route_tables_at(smem + buffers * kMoeWarps * stride * 16, args);
   const int strips = (args.I + kCols - 1) / kCols;
   const int by_index = static_cast<int>(gridDim.x) / strips, by_strip = static_cast<int>(gridDim.x) % strips;
   UnitCursor unit{static_cast<int>(blockIdx.x) / strips, static_cast<int>(blockIdx.x) % strips};
@@ -756,10 +762,11 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __gri
   build_route_tables(r, args);
   GateUp<W, F16> g{args, r, ptx::lane_id(), static_cast<int>(threadIdx.x) / 32, *r.count, {}};
   if (unit.index < g.experts && g.warp * kMoeStep < args.H) g.load(unit, g.warp * kMoeStep);
-  for (int turn = 0; unit.index < g.experts; turn ^= 1) {
+  for (int turn = 0; unit.index < g.experts; turn ^= buffers - 1) {
     UnitCursor next = unit;
     next.advance(strips, by_index, by_strip);
     g.run(red + turn * kMoeWarps * stride, stride, unit, next);
+    if (buffers == 1) __syncthreads();
     unit = next;
   }
 }

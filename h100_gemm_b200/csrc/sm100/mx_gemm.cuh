@@ -121,6 +121,12 @@ __device__ __forceinline__ float mx_finish(const MxGemmArgs& args, float acc) {
   return args.scale ? __fadd_rn(__fmul_rn(acc, args.alpha), args.beta) : acc;
 }
 
+// A bounded wait of a whole warp: one answer for all lanes, so that the warp stays converged whichever lane's budget
+// runs out first.
+__device__ __forceinline__ bool mx_warp_wait(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity));
+}
+
 // Grid: clusters of split * (1 or 2) CTAs. Pair p of a cluster takes K-tiles
 // [k_tiles * p / split, k_tiles * (p + 1) / split) of each of the cluster's tiles.
 template <int FMT, int BN, int PAIR, int F16>
@@ -263,14 +269,14 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
         // Separate ones: the tile before that, entirely.
         const bool wait_drained = T::kOverlap > 0 ? turn >= 1 : turn >= 2;
         const uint32_t drained_phase = static_cast<uint32_t>(T::kOverlap > 0 ? turn - 1 : turn / 2 - 1) & 1u;
-        if (wait_drained && !ptx::mbar_wait(drained_bar(T::kOverlap > 0 ? 0 : turn & 1), drained_phase)) {
+        if (wait_drained && !mx_warp_wait(drained_bar(T::kOverlap > 0 ? 0 : turn & 1), drained_phase)) {
           mx_report_timeout(args.status, kStatusMmaTmemTimeout, turn, 0, abort_flag);
           break;
         }
         const uint32_t tmem_d = tmem_base + ((turn & 1) ? T::kAcc1 : 0);
         for (int k_tile = 0; k_tile < len; ++k_tile) {
           // (the copies were issued after the stage had landed, so the second wait only orders this thread)
-          if (!ptx::mbar_wait(scales_bar(buffer), scales_phase) || !ptx::mbar_wait(full_bar(stage), phase)) {
+          if (!mx_warp_wait(scales_bar(buffer), scales_phase) || !mx_warp_wait(full_bar(stage), phase)) {
             mx_report_timeout(args.status, kStatusMmaFullTimeout, turn, k_tile, abort_flag);
             ok = false;
             break;
@@ -312,7 +318,7 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
       for (long long i = 0; i < total; ++i) {
         if (i >= T::kScaleBuffers) {
           // What the buffer holds, the scales of the K-tile kScaleBuffers before, must have been used.
-          if (!ptx::mbar_wait(empty_bar(old_stage), old_phase)) {
+          if (!mx_warp_wait(empty_bar(old_stage), old_phase)) {
             mx_report_timeout(args.status, kStatusMmaTmemTimeout, cluster, static_cast<int>(i), abort_flag);
             break;
           }
@@ -321,7 +327,7 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
             old_phase ^= 1u;
           }
         }
-        if (!ptx::mbar_wait(full_bar(stage), phase)) {
+        if (!mx_warp_wait(full_bar(stage), phase)) {
           mx_report_timeout(args.status, kStatusMmaFullTimeout, cluster, static_cast<int>(i), abort_flag);
           break;
         }
@@ -370,7 +376,7 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
       const int r_warp = tc.m * T::kTileRows + static_cast<int>(cta) * 128 + q * 32;  // this warp's first row
       const int row = r_warp + static_cast<int>(lane);
       const int s0 = tc.n * BN;
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(done_bar(acc), static_cast<uint32_t>(turn >> 1) & 1u))) {
+      if (!mx_warp_wait(done_bar(acc), static_cast<uint32_t>(turn >> 1) & 1u)) {
         if (lane == 0) mx_report_timeout(args.status, kStatusEpilogueTimeout, tile, acc, abort_flag);
         break;
       }
