@@ -47,15 +47,18 @@ int launch_all(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) 
   if (rc == B200_OK) rc = allow_shared_memory(dev, &moe_down_kernel<W, F16>, down_allowed);
   if (rc != B200_OK) return rc;
 
-  // One token alone has no company to share the router's rows with.
-  const int group = args.T == 1 ? 1 : kRouterTokens;
+  // As few tokens to a cluster as 8 clusters allow, which an idle device takes at once (4 tokens one to a cluster: 53.3 us
+  // for the layer, together 55.2); then up to kRouterTokens, so that the router's rows are not read too often.
+  const int group = args.T <= 8 ? 1 : args.T <= 16 ? 2 : kRouterTokens;
   const int clusters = (args.T + group - 1) / group;
   // 16 warps fill an SM with their registers: beyond 8 clusters two smaller CTAs per SM keep all of them resident
-  // (64 tokens, 128 experts: 8.4 against 10.5 us; 4 tokens: 6.8 against 6.1 us).
+  // (64 tokens, 128 experts: 8.4 against 10.5 us; 4 tokens in one cluster: 6.8 against 6.1 us).
   const int threads = clusters > 8 ? kRouterThreads / 2 : kRouterThreads;
   Launch route(clusters * kRouterCluster, threads, 0, stream, kRouterCluster);
   if (group == 1) {
     B200_TRY_CUDA(cudaLaunchKernelEx(&route.config, &moe_router_kernel<F16, 1>, args));
+  } else if (group == 2) {
+    B200_TRY_CUDA(cudaLaunchKernelEx(&route.config, &moe_router_kernel<F16, 2>, args));
   } else {
     B200_TRY_CUDA(cudaLaunchKernelEx(&route.config, &moe_router_kernel<F16, kRouterTokens>, args));
   }

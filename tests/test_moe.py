@@ -204,11 +204,12 @@ def test_nan_token_stays_alone():
 @pytest.mark.parametrize("fmt", [None, "mxfp4"])
 def test_tokens_do_not_depend_on_their_company(fmt):
     """A token's routing is the same alone and in a batch."""
-    x, router, w1, w2, *_ = make(30, 32, 512, 96, BF16, 8, fmt)
+    x, router, w1, w2, *_ = make(40, 32, 512, 96, BF16, 8, fmt)
     _, ids, weights = g.moe_layer(x, router, w1, w2, 4, return_routing=True)
     for t in (0, 7, 29):
-        _, one, w = g.moe_layer(x[t:t + 1].contiguous(), router, w1, w2, 4, return_routing=True)
-        assert torch.equal(one[0], ids[t]) and torch.equal(w[0], weights[t])
+        for n in (1, 2, 9, 11):
+            _, some, w = g.moe_layer(x[t:t + n].contiguous(), router, w1, w2, 4, return_routing=True)
+            assert torch.equal(some, ids[t:t + n]) and torch.equal(w, weights[t:t + n])
 
 
 @pytest.mark.gpu
