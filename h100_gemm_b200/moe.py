@@ -3,13 +3,21 @@ from __future__ import annotations
 
 from . import api
 from .api import STATUS_WORKSPACE, GemmError
-from .mx import FORMATS, MxTensor, _current, _elsewhere, _half_type, _invalid, _output, _require_cuda
+from .mx import FORMATS, MxTensor, _current, _elsewhere, _half_type, _invalid, _output, _require_cuda, _Torch
+
+torch = _Torch(globals())
 
 MAX_TOKENS, MAX_EXPERTS, MAX_TOP_K = 64, 512, 32
 
 
 def moe_workspace_bytes(tokens: int, experts: int, top_k: int, hidden: int, inner: int) -> int:
     return int(api.library().b200_moe_workspace_bytes(tokens, experts, top_k, hidden, inner))
+
+
+def _workspace_bytes(tokens: int, top_k: int, inner: int) -> int:
+    """b200_moe_workspace_bytes of sizes that are known to be within the limits."""
+    pairs = tokens * top_k
+    return (pairs * inner * 4 + 255) // 256 * 256 + (pairs * 4 + 255) // 256 * 512
 
 
 def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: bool = True, out=None,
@@ -26,7 +34,6 @@ def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: 
     logit first, -1 where fewer experts than top_k are left) and their weights (fp32). A token without any
     expert gets zeros. Expert weights have to be finite. include/b200_gemm.h has the rounding and the limits.
     """
-    import torch
     f16 = _half_type(x.dtype, "x")
     if x.dim() != 2 or router.dim() != 2 or router.shape[1] != x.shape[1]:
         raise _invalid("x must be [tokens, hidden] and router [experts, hidden]")
@@ -51,7 +58,7 @@ def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: 
         if w_gate_up.dim() != 3 or w_down.dim() != 3:
             raise _invalid("w_gate_up must be [experts, 2 I, hidden] and w_down [experts, hidden, I]")
         I = w_down.shape[2]
-        if tuple(w_gate_up.shape) != (E, 2 * I, H) or tuple(w_down.shape) != (E, H, I):
+        if w_gate_up.shape != (E, 2 * I, H) or w_down.shape != (E, H, I):
             raise _invalid(f"w_gate_up must be [{E}, 2 I, {H}] and w_down [{E}, {H}, I]")
     if H % 8 or I % 8 or H == 0 or I == 0:
         raise _invalid("hidden and inner sizes must be multiples of 8")
@@ -76,7 +83,7 @@ def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: 
         bias_ptr = pointer(bias, "bias", torch.float32, 4)
     if out is not None:
         _output(out, (T, H), dtype, device, True)
-    need = moe_workspace_bytes(T, E, top_k, H, I)
+    need = _workspace_bytes(T, top_k, I)
     if workspace is not None:
         _require_cuda(workspace.device, "workspace", device)
         if workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous():
@@ -99,7 +106,6 @@ def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: 
 
 
 def _launch(x, sizes, need, top_k, out, return_routing, workspace, handle):
-    import torch
     device = x.device
     if out is None:
         out = torch.empty_like(x)

@@ -21,6 +21,22 @@ import contextlib
 from . import api
 from .api import STATUS_INVALID_ARG, GemmError
 
+
+class _Torch:
+    """Stands for torch in a module until something of it is needed there: importing the package must not import it,
+    and an import statement in every call costs a quarter of a microsecond."""
+
+    def __init__(self, module: dict):
+        self._module = module
+
+    def __getattr__(self, name):
+        import torch
+        self._module["torch"] = torch
+        return getattr(torch, name)
+
+
+torch = _Torch(globals())
+
 FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
 _GROUPS = {"mxfp4": 2, "nvfp4": 4}  # 512-byte scale groups of a 128 x 256 tile
@@ -55,7 +71,6 @@ class MxTensor:
     __slots__ = ("rows", "cols", "format", "tensor_scale", "device", "_data", "_scales", "_pool", "_data_ptr", "_scales_ptr")
 
     def __init__(self, data, scales, rows: int, cols: int, format: str = "mxfp4", tensor_scale: float = 1.0):
-        import torch
         _format(format)
         if rows <= 0 or cols <= 0:
             raise _invalid("rows and cols must be positive")
@@ -81,7 +96,6 @@ class MxTensor:
     @classmethod
     def _empty(cls, rows: int, cols: int, format: str, tensor_scale: float, device) -> "MxTensor":
         """Uninitialised, in one allocation; the two tensors are made when somebody asks for them."""
-        import torch
         self = cls.__new__(cls)
         codes = rows * _pitch(cols)
         at = (codes + 255) // 256 * 256
@@ -111,7 +125,6 @@ class MxTensor:
     def from_parts(cls, codes, block_scales, cols: int, format: str = "mxfp4", tensor_scale: float = 1.0) -> "MxTensor":
         """Lays out weights that come as packed codes [rows, ceil(cols / 2)] and plain block scales
         [rows, ceil(cols / block)] (uint8 or the 8-bit float's own type), once."""
-        import torch
         _format(format)
         blocks = -(-cols // BLOCK[format])
         if codes.dim() != 2 or block_scales.dim() != 2 or codes.shape[1] != (cols + 1) // 2 or \
@@ -143,7 +156,6 @@ class MxTensor:
 def _elsewhere(device, stream):
     """Another device than the current one, or a stream of the caller's choice: memory is allocated there, in
     that stream's order."""
-    import torch
     with torch.cuda.device(device):
         if stream is None:
             yield torch.cuda.current_stream().cuda_stream or None
@@ -161,9 +173,10 @@ def _elsewhere(device, stream):
 
 def _current(device, stream):
     """The current stream's handle where a call can run as it is, the usual case; else False (see _elsewhere)."""
-    import torch
-    if stream is None and torch.cuda.current_device() == device.index:
-        return torch._C._cuda_getCurrentRawStream(device.index) or None
+    if stream is None:
+        index = device.index
+        if torch._C._cuda_getDevice() == index:
+            return torch._C._cuda_getCurrentRawStream(index) or None
     return False
 
 
@@ -175,7 +188,6 @@ def _require_cuda(device, name: str, expected=None):
 
 
 def _half_type(dtype, name: str) -> int:
-    import torch
     if dtype is torch.bfloat16:
         return 0
     if dtype is torch.float16:
@@ -250,13 +262,12 @@ def quantize_mx_both(x, format: str = "mxfp4", tensor_scale: float = 1.0, stream
 
 def _output(out, shape, dtype, device, contiguous: bool) -> None:
     _require_cuda(out.device, "out", device)
-    if out.dtype is not dtype or tuple(out.shape) != shape or (contiguous and not out.is_contiguous()):
+    if out.dtype is not dtype or out.shape != shape or (contiguous and not out.is_contiguous()):
         raise _invalid(f"out must be a {'contiguous ' if contiguous else ''}{list(shape)} {dtype} tensor")
 
 
 def dequantize_mx(q: MxTensor, dtype=None, out=None, stream=None):
     """The values of q as a [rows, cols] bf16 (default) or fp16 tensor."""
-    import torch
     if not isinstance(q, MxTensor):
         raise _invalid(f"q must be an MxTensor, got {type(q).__name__}")
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
@@ -275,7 +286,6 @@ def dequantize_mx(q: MxTensor, dtype=None, out=None, stream=None):
 
 
 def _launch_dequantize(q, dtype, f16, out, ld, handle):
-    import torch
     if out is None:
         out = torch.empty(q.rows, q.cols, dtype=dtype, device=q.device)
     rc = api.library().b200_mx_dequantize(FORMATS[q.format], f16, q.rows, q.cols, q._data_ptr, q._scales_ptr, q.tensor_scale,
@@ -288,7 +298,6 @@ def _launch_dequantize(q, dtype, f16, out, ld, handle):
 def gemm_mx(a: MxTensor, b: MxTensor, out=None, alpha: float = 1.0, beta: float = 0.0, dtype=None, stream=None):
     """out[M, N] = (a[M, K] @ b[N, K]^T) * alpha + beta for two 4-bit matrices of one format, tensor scales
     applied; bf16 (default) or fp16 output, fp32 accumulation."""
-    import torch
     if not isinstance(a, MxTensor) or not isinstance(b, MxTensor):
         raise _invalid(f"a and b must be MxTensors, got {type(a).__name__} and {type(b).__name__}")
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
@@ -311,7 +320,6 @@ def gemm_mx(a: MxTensor, b: MxTensor, out=None, alpha: float = 1.0, beta: float 
 
 
 def _launch_gemm(a, b, dtype, f16, out, alpha, beta, handle):
-    import torch
     if out is None:
         out = torch.empty(a.rows, b.rows, dtype=dtype, device=a.device)
     rc = api.library().b200_gemm_mx(FORMATS[a.format], f16, a.rows, b.rows, a.cols, a._data_ptr, a._scales_ptr, b._data_ptr,

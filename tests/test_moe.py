@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import h100_gemm_b200 as g
-from h100_gemm_b200 import api
+from h100_gemm_b200 import api, moe
 from test_mx import random_mx
 
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -103,6 +103,8 @@ def test_workspace_and_refusals_without_a_device():
     for bad in ((0, 8, 2, 64, 64), (65, 8, 2, 64, 64), (1, 513, 2, 64, 64), (1, 8, 9, 64, 64), (1, 64, 33, 64, 64),
                 (1, 8, 0, 64, 64), (1, 8, 2, 60, 64), (1, 8, 2, 64, 0)):
         assert g.moe_workspace_bytes(*bad) == 0
+    for T, k, I in ((1, 1, 8), (3, 5, 40), (64, 32, 1000), (17, 3, 768), (8, 8, 64)):
+        assert moe._workspace_bytes(T, k, I) == g.moe_workspace_bytes(T, 40, k, 64, I)
     z = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype)  # noqa: E731
     good = dict(x=z(2, 64), router=z(8, 64), w_gate_up=z(8, 64, 64), w_down=z(8, 64, 32), top_k=2)
     for change, text in ((dict(), "CUDA tensor"), (dict(x=z(2, 64, dtype=torch.float32)), "bfloat16 or float16"),
