@@ -625,7 +625,7 @@ struct MoeStep {
   }
 };
 
-B200_DEVICE float silu(float v) { return __fdividef(v, 1.0f + __expf(-v)); }
+B200_DEVICE float silu(float v) { return __fdiv_rn(v, 1.0f + expf(-v)); }
 
 // The tokens of an expert ride on the MMA's N in the order of its pairs, two n-tiles at a time (more would
 // need more registers than the weights leave). Columns beyond the last token repeat it and are not used.
@@ -731,7 +731,9 @@ struct GateUp {
       uint16_t* to = args.h + static_cast<long long>(r.pairs[first_pair + c]) * 2 * args.I + row;
       const uint16_t nearest = round16<F16>(h);
       to[0] = nearest;
-      to[args.I] = round16<F16>(h - widen16<F16>(nearest));  // (NaN where h is infinite: the sum is not finite either way)
+      // (beyond the type's range h becomes infinite, as it would in one part, and not the NaN of inf - inf)
+      const float rest = h - widen16<F16>(nearest);
+      to[args.I] = round16<F16>(isinf(rest) || isinf(h) ? 0.0f : rest);
     }
   }
 };

@@ -203,6 +203,20 @@ def test_nan_token_stays_alone():
 
 
 @pytest.mark.gpu
+def test_hidden_values_beyond_fp16():
+    """A hidden value of 10^5 is infinite in fp16, and so is what the down product makes of it; one of 60000 is not."""
+    x = torch.full((2, 64), 1.0, dtype=FP16, device="cuda")
+    x[1] = 0.75
+    w1 = torch.zeros(1, 16, 64, dtype=FP16, device="cuda")
+    w1[0, :8], w1[0, 8:] = 1000.0 / 64, 100.0 / 64             # gate 1000 and up 100, or 750 and 75
+    w2 = torch.full((1, 64, 8), 1.0 / 16, dtype=FP16, device="cuda")
+    out = g.moe_layer(x, torch.zeros(1, 64, dtype=FP16, device="cuda"), w1, w2, 1)
+    assert (out[0] == math.inf).all()
+    want = 8 * 750.0 * 75.0 / 16                                  # every number on the way is exact to 2^-11
+    assert ((out[1].double() - want).abs() <= 4 * 2.0 ** -11 * want).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", [None, "mxfp4"])
 def test_tokens_do_not_depend_on_their_company(fmt):
     """A token's routing is the same alone and in a batch."""
