@@ -285,7 +285,6 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   volatile uint32_t* abort_flag = tmem_ptr_slot + 1;
 
   // ---------------------------------------------------------------- set-up
-  ptx::grid_launch_dependents();  // the next kernel in the stream may begin its own set-up
   if (warp == 0 && lane == 0) {
     ptx::prefetch_tensormap(&map_a);
     ptx::prefetch_tensormap(&map_b);
@@ -313,6 +312,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   }
   ptx::tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_ptr_slot;
+  // The next kernel in the stream may begin its own set-up. Not before this CTA has its tensor memory: a CTA of a
+  // smaller kernel beside it (a 4-bit product) could otherwise take the columns first and wait for this grid, which
+  // would wait for the columns.
+  ptx::grid_launch_dependents();
   // Programmatic dependent launch: everything above (barriers, tensor memory, descriptor prefetch)
   // may overlap the tail of the previous kernel in the stream; nothing below may, because it reads
   // or writes global memory that kernel may still be using (operands, C, partial tiles, flags).
