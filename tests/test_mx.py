@@ -536,6 +536,43 @@ def test_quantise_rows_at_every_offset(offset, dtype, fmt):
 
 
 @pytest.mark.gpu
+def test_between_products_with_short_rings():
+    """A 16-bit product of two stages leaves an SM room for a 4-bit one beside it: both need tensor memory, and each
+    begins while the other still runs. Captured, so that nothing but the kernels keeps them in order."""
+    gen = torch.Generator().manual_seed(8)
+    a = torch.randn(700, 512, generator=gen).bfloat16().cuda()
+    b = (torch.randn(512, 512, generator=gen) * 512 ** -0.5).bfloat16().cuda()
+    cfg = api.GemmConfig(block_n=256, cluster_m=1, stages=2)
+    w, small = g.quantize_mx(b), g.quantize_mx(a[:20])
+
+    def chain():
+        outs = []
+        x = a
+        for _ in range(6):
+            x = g.gemm(x, b, cfg=cfg)
+            outs += [x, g.gemm_mx(small, w), g.gemm_mx(g.quantize_mx(x), w)]
+        return outs
+
+    want = []
+    x = a
+    for _ in range(6):
+        x = g.gemm(x, b, cfg=cfg)
+        torch.cuda.synchronize()
+        q = g.quantize_mx(x)
+        torch.cuda.synchronize()
+        want += [x, g.gemm_mx(small, w), g.gemm_mx(q, w)]
+        torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = chain()
+    for _ in range(20):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w_) for o, w_ in zip(got, want))
+    assert g.device_status()[0] == api.STATUS_OK
+
+
+@pytest.mark.gpu
 def test_two_streams_at_once():
     """Passes on two streams without any wait between them: nothing is shared."""
     gen = torch.Generator().manual_seed(6)
