@@ -89,10 +89,14 @@ B200_DEVICE void setmaxnreg_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
 }
 
+// Cluster barrier. The aligned forms want all lanes of a warp at the instruction together, which nothing else promises
+// after a loop whose trip count differs between lanes: so the lanes meet here, whatever the caller did before.
 B200_DEVICE void cluster_arrive() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 }
 B200_DEVICE void cluster_wait() {
+  __syncwarp();
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
