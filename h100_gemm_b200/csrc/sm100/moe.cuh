@@ -179,7 +179,9 @@ __global__ void __launch_bounds__(kRouterThreads) moe_router_kernel(const __grid
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
       if (lane == 0 && j < tokens) {
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(ptx::map_to_cta(logits_addr + e * 4, j)), "f"(s + bias)
+        // (an expert that is masked out stays out, whatever its product is: NaN + -inf would be a NaN, the first choice)
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(ptx::map_to_cta(logits_addr + e * 4, j)),
+                     "f"(bias == -INFINITY ? bias : s + bias)
                      : "memory");
       }
     }

@@ -304,7 +304,8 @@ int b200_gemm_mx(int format, int f16, int M, int N, int K, const void* A, const 
 
 /* A mixture-of-experts layer for a few tokens (a decode step), from the router to the weighted sum. No
  * counterpart in the reference.
- *   l[t, e] = X[t] . router[e] + bias[e]                  fp32; bias may be NULL, -inf takes an expert out
+ *   l[t, e] = X[t] . router[e] + bias[e]                  fp32; bias may be NULL, -inf takes an expert out, whatever its
+ *             product is (an infinity or a NaN included)
  *   S[t]    = the top_k largest l[t, .], ties to the lower index, -inf never chosen, NaN before all others
  *   p[t, e] = exp(l[t, e]) / sum of exp(l[t, .]) over S[t] (renormalize) or over all experts
  *   h[t, e] = p[t, e] silu(W1[e, 0 : I] X[t]) (W1[e, I : 2 I] X[t])      fp32, kept in two parts of the type of X
