@@ -63,7 +63,8 @@ int launch_all(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) 
     B200_TRY_CUDA(cudaLaunchKernelEx(&route.config, &moe_router_kernel<F16, kRouterTokens>, args));
   }
 
-  constexpr int MT = MoeUnit<W>::kTiles;
+  constexpr int MT = MoeUnit<W, F16>::kTiles;
+  using Hidden = Down<W, F16>;
   const int tables = route_table_bytes(args.E, args.T * args.k);
   const int most = args.T * args.k < args.E ? args.T * args.k : args.E;  // experts that can be chosen
   const long long units = static_cast<long long>(most) * ((args.I + 8 * MT - 1) / (8 * MT));
@@ -72,11 +73,11 @@ int launch_all(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) 
   B200_TRY_CUDA(cudaLaunchKernelEx(&up.config, &moe_gate_up_kernel<W, F16>, args));
 
   // Clusters share the columns of a unit until every SM has two CTAs, but no warp is left without a step.
-  const int columns = (args.H + 16 * MT - 1) / (16 * MT);
-  const long long steps = static_cast<long long>(most) * ((args.I + kMoeStep - 1) / kMoeStep);
+  const int columns = (args.H + 16 * Hidden::MT - 1) / (16 * Hidden::MT);
+  const long long steps = static_cast<long long>(most) * ((args.I + Hidden::kStep - 1) / Hidden::kStep);
   int split = 1;
   while (split < 8 && columns * split * 2 <= dev.sm_count * 2 && steps >= 2ll * split * kMoeWarps) split *= 2;
-  Launch down(columns * split, kMoeThreads, (kMoeWarps * args.T * Down<W, F16>::kPitch * 4 + 15) / 16 * 16 + tables, stream,
+  Launch down(columns * split, kMoeThreads, (kMoeWarps * args.T * Hidden::kPitch * 4 + 15) / 16 * 16 + tables, stream,
               split);
   B200_TRY_CUDA(cudaLaunchKernelEx(&down.config, &moe_down_kernel<W, F16>, args, split));
   return B200_OK;
@@ -130,7 +131,7 @@ int b200_moe_layer(int f16, int T, int E, int top_k, int H, int I, const void* X
   args.w2.scales = static_cast<const uint8_t*>(W2_scales);
   args.w2.pitch = four_bit ? mx_pitch(I) : 2ll * I;
   args.w2.col_tiles = mx_col_tiles(I);
-  const float lift = weight_format == B200_NVFP4 ? MoeUnit<kMoeNvfp4>::kLift : 1.0f;
+  const float lift = weight_format == B200_NVFP4 ? MoeUnit<kMoeNvfp4, 0>::kLift : 1.0f;
   args.lift1 = four_bit ? lift * W1_tensor_scale : 1.0f;
   args.lift2 = four_bit ? lift * W2_tensor_scale : 1.0f;
   args.h = reinterpret_cast<uint16_t*>(ws);

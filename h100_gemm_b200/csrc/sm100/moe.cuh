@@ -3,13 +3,12 @@
 //   logits  l[t, e] = x[t] . R[e] + b[e]                                        (fp32)
 //   chosen  S[t] = the k largest logits of t (ties: the lower index; -inf is never chosen)
 //   weight  p[t, e] = exp(l[t, e]) / sum of exp(l) over S[t], or over all experts
-//   gated   h[t, e] = p[t, e] * silu(G_e x[t]) * (U_e x[t])                     (fp32, kept in two 16-bit parts)
+//   gated   h[t, e] = p[t, e] * silu(G_e x[t]) * (U_e x[t])                     (fp32)
 //   out[t] = sum over e in S[t] of D_e h[t, e]                                  (fp32, rounded once)
 //
-// (The routing weight goes into h, so the down product of all experts of a token is a single sum. h is kept as
-// its nearest 16-bit number and the nearest 16-bit number of what that leaves, 16 bits of bf16 or 22 of fp16: one
-// part alone costs the result a second rounding, an error 1.4 times as large. The two parts ride side by side on
-// columns of the MMA that a decode step leaves empty anyway.)
+// (The routing weight goes into h, so the down product of all experts of a token is a single sum. The tensor cores take
+// 16-bit operands, so h meets the down weights in parts (HiddenParts), 22 bits of it for bf16: outputs then differ from
+// those of an fp32 hidden value as seldom as fp32 sums in another order do.)
 //
 // Bound by memory: every chosen expert's 3 H I weights are read once and used for a handful of
 // tokens. So the weights go straight from global memory to registers in the shape of an MMA's A
@@ -24,8 +23,6 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include <type_traits>
-
 #include "mx_format.cuh"
 #include "ptx.cuh"
 
@@ -36,7 +33,6 @@ static constexpr int kMoeMaxExperts = 512;
 static constexpr int kMoeMaxTopK = 32;
 static constexpr int kMoeThreads = 256;
 static constexpr int kMoeWarps = kMoeThreads / 32;
-static constexpr int kMoeStep = 256;         // elements of the contraction one warp takes at a time
 static constexpr int kRouterCluster = 8;
 static constexpr int kRouterThreads = 512;  // at most
 static constexpr int kRouterTokens = 4;      // tokens one cluster routes, at most
@@ -62,7 +58,7 @@ struct MoeArgs {
   float lift1, lift2;       // what sums of products with w1 / w2 are multiplied with (1 for 16-bit weights)
   int* ids;                 // [T, k], -1 = none
   float* weights;           // [T, k]
-  uint16_t* h;              // [T, k, 2, I]
+  uint16_t* h;              // [T, k, 2, I]: HiddenParts
   uint16_t* out;            // [T, H]
 };
 
@@ -106,6 +102,129 @@ B200_DEVICE uint16_t round16(float v) {
   } else {
     return __bfloat16_as_ushort(__float2bfloat16_rn(v));
   }
+}
+
+B200_DEVICE uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+B200_DEVICE uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
+// ------------------------------------------------------------------------------------- hidden values
+// A hidden value takes two 16-bit words, in two planes, and meets the weights in kParts operands whose sums are scaled and
+// added. Its elements lie in the order that the weights' MMA takes them in (hidden_place).
+//
+// bf16: the fp32 number, rounded to 22 significant bits: its upper half, and the next two groups of 7 bits, m1 below m2. With
+// E = +-2^e, sign and exponent alone, the parts are the upper half itself, E * m1 / 128 and E * m2 / 128: each
+// exact in bf16 and two or three instructions for two elements (E | m is E + E m / 128).
+// fp16: the nearest fp16 number, and the nearest one of what that leaves.
+template <int F16>
+struct HiddenParts;
+
+template <>
+struct HiddenParts<0> {
+  static constexpr int kParts = 3;
+  static B200_DEVICE float factor(int p) { return p == 0 ? 1.0f : p == 1 ? 0.0078125f : 0.00006103515625f; }  // 1, 2^-7, 2^-14
+  static B200_DEVICE void store(float h, uint16_t* first, uint16_t* second) {
+    const uint32_t bits = h == h ? __float_as_uint(h) + 2u : 0x7FC00000u;  // (beyond the largest number: infinity)
+    *first = static_cast<uint16_t>(bits >> 16);
+    *second = static_cast<uint16_t>((bits >> 9 & 0x7Fu) | (bits >> 2 & 0x7Fu) << 8);
+  }
+  static B200_DEVICE uint32_t lower(uint32_t first, uint32_t m) {
+    const uint32_t e = first & 0xFF80FF80u;
+    return sub_bf16x2((m & 0x007F007Fu) | e, e);
+  }
+  static B200_DEVICE void all(uint32_t (&part)[kParts], uint32_t first, uint32_t second) {
+    part[0] = first;
+    part[1] = lower(first, second);
+    part[2] = lower(first, second >> 8);
+  }
+  // Part `p`, the same for all elements of a lane.
+  static constexpr int kReads = 2;
+  static B200_DEVICE uint32_t one(const uint32_t (&word)[kReads], int p) {
+    const uint32_t v = lower(word[0], word[1] >> (p == 2 ? 8 : 0));
+    return p == 0 ? word[0] : v;
+  }
+};
+
+template <>
+struct HiddenParts<1> {
+  static constexpr int kParts = 2;
+  static B200_DEVICE float factor(int) { return 1.0f; }
+  static B200_DEVICE void store(float h, uint16_t* first, uint16_t* second) {
+    *first = round16<1>(h);
+    // (beyond the type's range h becomes infinite, as it would in one part, and not the NaN of inf - inf)
+    const float rest = h - widen16<1>(*first);
+    *second = round16<1>(isinf(rest) || isinf(h) ? 0.0f : rest);
+  }
+  static B200_DEVICE void all(uint32_t (&part)[kParts], uint32_t first, uint32_t second) {
+    part[0] = first;
+    part[1] = second;
+  }
+  static constexpr int kReads = 1;  // of the part's own plane
+  static B200_DEVICE uint32_t one(const uint32_t (&word)[kReads], int) { return word[0]; }
+};
+
+// How the columns of an MMA take hidden vectors (`base`: the first plane, `plane` elements before the second).
+// HiddenSums: column g is a token, its parts go to kSums accumulators one after the other. HiddenColumns: the parts of a token
+// lie side by side on kWidth columns (of bf16's four one is idle), with one accumulator and a third of the MMAs. An expert
+// with as few tokens as one tile of those holds takes them: 4 tokens 54.2 us against 57.8 with sums alone, 16 tokens
+// 123.4 against 130, 4 tokens MXFP4 40.3 against 43. (Two such tiles at once for 3 and 4 tokens: 16 tokens 122 us, but 64
+// tokens of 4-bit experts 176 against 155, a third variant of the unrolled product being too much code.)
+template <int F16>
+struct HiddenSums {
+  using P = HiddenParts<F16>;
+  static constexpr int kSums = P::kParts, kReads = 2, kTokens = 8;
+  const uint16_t* at[kReads];
+  B200_DEVICE HiddenSums(const uint16_t* base, int plane, int) : at{base, base + plane} {}
+  B200_DEVICE void operands(uint32_t (&b)[kSums][4], const uint4 (&v)[kReads]) const {
+    const uint32_t first[4] = {v[0].x, v[0].y, v[0].z, v[0].w}, second[4] = {v[1].x, v[1].y, v[1].z, v[1].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t part[kSums];
+      P::all(part, first[i], second[i]);
+#pragma unroll
+      for (int p = 0; p < kSums; ++p) b[p][i] = part[p];
+    }
+  }
+};
+
+template <int F16>
+struct HiddenColumns {
+  using P = HiddenParts<F16>;
+  static constexpr int kWidth = P::kParts == 3 ? 4 : 2;
+  static constexpr int kSums = 1, kReads = P::kReads, kTokens = 8 / kWidth;
+  const uint16_t* at[kReads];
+  int part;
+  B200_DEVICE HiddenColumns(const uint16_t* base, int plane, int column) : part(column % kWidth) {
+    at[0] = kReads == 1 ? base + part * plane : base;
+    if constexpr (kReads == 2) at[1] = base + plane;
+  }
+  B200_DEVICE void operands(uint32_t (&b)[1][4], const uint4 (&v)[kReads]) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t word[kReads];
+#pragma unroll
+      for (int r = 0; r < kReads; ++r) word[r] = i == 0 ? v[r].x : i == 1 ? v[r].y : i == 2 ? v[r].z : v[r].w;
+      b[0][i] = P::one(word, part);
+    }
+  }
+};
+
+// The parts' sums as one. Where an infinite or NaN hidden value makes the first sum that, the others hold inf - inf: the first
+// alone is what the formula gives.
+template <int F16>
+B200_DEVICE float join_parts(const float (&sum)[HiddenParts<F16>::kParts]) {
+  float v = sum[0];
+#pragma unroll
+  for (int p = 1; p < HiddenParts<F16>::kParts; ++p) v = fmaf(sum[p], HiddenParts<F16>::factor(p), v);
+  return isfinite(sum[0]) ? v : sum[0];
 }
 
 // ------------------------------------------------------------------------------------- router
@@ -382,14 +501,15 @@ B200_DEVICE void build_route_tables(const RouteTables& r, const MoeArgs& args) {
 }
 
 // ------------------------------------------------------------------------------------- weights in registers
-// One warp's share of a step: MT x 16 weight rows against kMoeStep elements from k0 on. Row g of MMA m
-// is `rows(m, 0)`, row g + 8 is `rows(m, 1)` (negative: zeros). load() only issues the loads; mma() multiplies with
-// one n-tile, whose column g is the vector `b`.
+// One warp's share of a step: MT x 16 weight rows against kStep elements of the contraction from k0 on. Row g of MMA m
+// is `rows(m, 0)`, row g + 8 is `rows(m, 1)` (negative: zeros). load() only issues the loads; mma_tokens() multiplies
+// with n-tiles whose column g is the vector `b[j]`, mma_hidden() with one of hidden values.
 //
-// 16-bit weights: eight chunks of 32 elements, a lane 16 bytes of each row and chunk.
-template <int W, int F16, int MT>
+// 16-bit weights: CHUNKS times 32 elements, a lane 16 bytes of each row and chunk.
+template <int F16, int MT, int CHUNKS>
 struct WeightStep {
-  uint4 q[MT][2][8];
+  static constexpr int kStep = CHUNKS * 32;
+  uint4 q[MT][2][CHUNKS];
 
   template <typename Rows>
   B200_DEVICE void load(const MoeMatrix& w, int k0, int K, uint32_t lane, Rows rows) {
@@ -400,12 +520,12 @@ struct WeightStep {
       for (int half = 0; half < 2; ++half) {
         const int row = rows(m, half);
         const uint8_t* p = w.data + row * w.pitch + kl * 2;
-        if (row >= 0 && k0 + kMoeStep <= K) {
+        if (row >= 0 && k0 + kStep <= K) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) q[m][half][c] = ptx::ld_stream_v4(p + c * 64);
+          for (int c = 0; c < CHUNKS; ++c) q[m][half][c] = ptx::ld_stream_v4(p + c * 64);
         } else {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
+          for (int c = 0; c < CHUNKS; ++c) {
             q[m][half][c] = make_uint4(0u, 0u, 0u, 0u);
             if (row >= 0 && kl + c * 32 < K) q[m][half][c] = ptx::ld_stream_v4(p + c * 64);
           }
@@ -417,9 +537,9 @@ struct WeightStep {
   B200_DEVICE void mma(float (&acc)[MT][4], const uint16_t* b, int k0, int K, uint32_t lane) const {
     const int kl = k0 + static_cast<int>(lane & 3u) * 8;
 #pragma unroll
-    for (int c0 = 0; c0 < 8; c0 += 4) {  // (all eight at once would spill)
+    for (int c0 = 0; c0 < CHUNKS; c0 += 4) {  // (eight at once would spill)
       uint4 v[4];
-      if (k0 + kMoeStep <= K) {
+      if (k0 + kStep <= K) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) v[c] = *reinterpret_cast<const uint4*>(b + kl + (c0 + c) * 32);
       } else {
@@ -440,15 +560,48 @@ struct WeightStep {
       }
     }
   }
+
+  template <int NT>
+  B200_DEVICE void mma_tokens(float (&acc)[NT][MT][4], const uint16_t* const (&b)[NT], int k0, int K, uint32_t lane) const {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) mma(acc[j], b[j], k0, K, lane);
+  }
+
+  static B200_DEVICE int hidden_place(int i) { return i; }
+  template <typename Hidden>
+  B200_DEVICE void mma_hidden(float (&acc)[Hidden::kSums][MT][4], const Hidden& columns, int k0, int K, uint32_t lane) const {
+    const int kl = k0 + static_cast<int>(lane & 3u) * 8;
+#pragma unroll
+    for (int c0 = 0; c0 < CHUNKS; c0 += 2) {
+      uint4 v[2][Hidden::kReads];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int at = kl + (c0 + c) * 32;
+#pragma unroll
+        for (int r = 0; r < Hidden::kReads; ++r) {
+          v[c][r] = make_uint4(0u, 0u, 0u, 0u);
+          if (k0 + kStep <= K || at < K) v[c][r] = *reinterpret_cast<const uint4*>(columns.at[r] + at);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t b[Hidden::kSums][4];
+        columns.operands(b, v[c]);
+#pragma unroll
+        for (int j = 0; j < Hidden::kSums; ++j) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const uint4 &lo = q[m][0][c0 + c], &hi = q[m][1][c0 + c];
+            mma16816<F16>(acc[j][m], lo.x, hi.x, lo.y, hi.y, b[j][0], b[j][1]);
+            mma16816<F16>(acc[j][m], lo.z, hi.z, lo.w, hi.w, b[j][2], b[j][3]);
+          }
+        }
+      }
+    }
+  }
 };
 
-B200_DEVICE uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-
-// 4-bit weights: two chunks of 128 elements, a lane 16 bytes = 32 elements of each row and chunk.
+// 4-bit weights: CHUNKS times 128 elements, a lane 16 bytes = 32 elements of each row and chunk.
 //
 // Unpacking, not memory, is what this kernel spends most instructions on. A code's magnitude bits at the top of a
 // bf16 number's mantissa and the bottom of its exponent read code * 2^-126. Of a word's eight codes, i and
@@ -459,12 +612,13 @@ B200_DEVICE uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 // scale above 2 (byte > 128) would leave bf16's range and takes a second one; a step that has any, or a NaN scale,
 // goes the general way.
 static constexpr float kNvfp4Lift = 65536.0f;
-template <int W, int MT>
+template <int W, int MT, int CHUNKS>
 struct WeightStep4 {
+  static constexpr int kStep = CHUNKS * 128;
   static constexpr int FMT = W == kMoeMxfp4 ? kMxfp4 : kNvfp4;
   static constexpr int kBlocks = 32 / mx_block(FMT);  // block scales of a lane's 32 elements
-  uint4 q[MT][2][2];
-  uint32_t sb[MT][2][2];
+  uint4 q[MT][2][CHUNKS];
+  uint32_t sb[MT][2][CHUNKS];
 
   template <typename Rows>
   B200_DEVICE void load(const MoeMatrix& w, int k0, int K, uint32_t lane, Rows rows) {
@@ -473,7 +627,6 @@ struct WeightStep4 {
     const uint8_t* codes = w.data + k0 / 2 + part * 16;
     const uint8_t* scales = w.scales + (block / 4) * kMxGroupBytes + block % 4;
     const long long tile_row = w.col_tiles * mx_tile_bytes(FMT);
-    const bool live0 = k0 + static_cast<int>(part) * 32 < K, live1 = k0 + 128 + static_cast<int>(part) * 32 < K;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -483,10 +636,10 @@ struct WeightStep4 {
         const uint8_t* p = codes + row * w.pitch;
         const uint8_t* sp = scales + (row / kMxTileRows) * tile_row + (row % 32) * 16 + (row % kMxTileRows) / 32 * 4;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < CHUNKS; ++c) {
           q[m][half][c] = make_uint4(0u, 0u, 0u, 0u);
           sb[m][half][c] = 0u;
-          if (signed_row >= 0 && (c == 0 ? live0 : live1)) {
+          if (signed_row >= 0 && k0 + c * 128 + static_cast<int>(part) * 32 < K) {
             q[m][half][c] = ptx::ld_stream_v4(p + c * 64);
             if constexpr (FMT == kMxfp4) {
               sb[m][half][c] = sp[c * kMxGroupBytes];
@@ -534,13 +687,14 @@ struct WeightStep4 {
     }
   }
 
-  // NT n-tiles at once, so that a weight is unpacked once: column g of tile j is the vector b[j]. GENERAL: any
-  // scale, and a step that the end of the rows may cut short.
-  template <int NT, bool GENERAL>
-  B200_DEVICE void mma(float (&acc)[NT][MT][4], const uint16_t* const (&b)[NT], int k0, int K, uint32_t lane) const {
+  // NT sums at once, so that a weight is unpacked once: `columns` makes their operands, eight elements as four pairs, of
+  // the eight 16-bit words that lie at each of its vectors. GENERAL: any scale, and a step that the end of the
+  // rows may cut short.
+  template <bool GENERAL, int NT, typename Columns>
+  B200_DEVICE void products(float (&acc)[NT][MT][4], const Columns& columns, int k0, int K, uint32_t lane) const {
     const int part = static_cast<int>(lane & 3u);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < CHUNKS; ++c) {
       const int kc = k0 + c * 128 + part * 32;
       uint32_t first[MT][2][kBlocks], second[MT][2][kBlocks];
 #pragma unroll
@@ -553,11 +707,11 @@ struct WeightStep4 {
       }
 #pragma unroll
       for (int word = 0; word < 4; ++word) {
-        uint4 v[NT];
+        uint4 v[Columns::kReads];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int j = 0; j < Columns::kReads; ++j) {
           if constexpr (GENERAL) v[j] = make_uint4(0u, 0u, 0u, 0u);
-          if (!GENERAL || kc + word * 8 < K) v[j] = *reinterpret_cast<const uint4*>(b[j] + kc + word * 8);
+          if (!GENERAL || kc + word * 8 < K) v[j] = *reinterpret_cast<const uint4*>(columns.at[j] + kc + word * 8);
         }
         uint32_t a[MT][2][4];
         const int i = kBlocks == 2 ? word / 2 : 0;
@@ -570,18 +724,56 @@ struct WeightStep4 {
                             second[m][half][i]);
           }
         }
+        uint32_t b[NT][4];
+        columns.operands(b, v);
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
-          const uint32_t b0 = __byte_perm(v[j].x, v[j].z, 0x5410), b1 = __byte_perm(v[j].x, v[j].z, 0x7632);
-          const uint32_t b2 = __byte_perm(v[j].y, v[j].w, 0x5410), b3 = __byte_perm(v[j].y, v[j].w, 0x7632);
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
-            mma16816<0>(acc[j][m], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], b0, b1);
-            mma16816<0>(acc[j][m], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], b2, b3);
+            mma16816<0>(acc[j][m], a[m][0][0], a[m][1][0], a[m][0][1], a[m][1][1], b[j][0], b[j][1]);
+            mma16816<0>(acc[j][m], a[m][0][2], a[m][1][2], a[m][0][3], a[m][1][3], b[j][2], b[j][3]);
           }
         }
       }
     }
+  }
+
+  // Column g of tile j is the vector at[j], element after element.
+  template <int NT>
+  struct Tokens {
+    static constexpr int kReads = NT;
+    const uint16_t* at[NT];
+    B200_DEVICE void operands(uint32_t (&b)[NT][4], const uint4 (&v)[NT]) const {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        b[j][0] = __byte_perm(v[j].x, v[j].z, 0x5410);
+        b[j][1] = __byte_perm(v[j].x, v[j].z, 0x7632);
+        b[j][2] = __byte_perm(v[j].y, v[j].w, 0x5410);
+        b[j][3] = __byte_perm(v[j].y, v[j].w, 0x7632);
+      }
+    }
+  };
+  // Elements i and i + 4 of eight side by side, as unpack() leaves the weights.
+  static B200_DEVICE int hidden_place(int i) { return (i & ~7) | (i & 3) << 1 | (i >> 2 & 1); }
+
+  template <int NT, typename Columns>
+  B200_DEVICE void mma(float (&acc)[NT][MT][4], const Columns& columns, int k0, int K, uint32_t lane) const {
+    if (k0 + kStep > K || general()) {
+      products<true>(acc, columns, k0, K, lane);
+    } else {
+      products<false>(acc, columns, k0, K, lane);
+    }
+  }
+  template <int NT>
+  B200_DEVICE void mma_tokens(float (&acc)[NT][MT][4], const uint16_t* const (&b)[NT], int k0, int K, uint32_t lane) const {
+    Tokens<NT> columns;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) columns.at[j] = b[j];
+    mma(acc, columns, k0, K, lane);
+  }
+  template <typename Hidden>
+  B200_DEVICE void mma_hidden(float (&acc)[Hidden::kSums][MT][4], const Hidden& columns, int k0, int K, uint32_t lane) const {
+    mma(acc, columns, k0, K, lane);
   }
 
   B200_DEVICE bool general() const {
@@ -589,8 +781,8 @@ struct WeightStep4 {
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t bytes = sb[m][i / 2][i % 2];
+      for (int i = 0; i < 2 * CHUNKS; ++i) {
+        const uint32_t bytes = sb[m][i / CHUNKS][i % CHUNKS];
         if constexpr (W == kMoeMxfp4) {
           some = some || bytes > 128u;
         } else {
@@ -602,35 +794,36 @@ struct WeightStep4 {
   }
 };
 
-// MMA tiles of weight rows a unit has: 4-bit rows are a quarter as long, so a unit takes two to keep as much on the way.
-template <int W>
+// MMA tiles of weight rows and steps of the two products: 8 KB on the way per warp, or 4 KB of 4-bit weights, whose rows are a
+// quarter as long, so that a unit takes two tiles. 16-bit weights do so in the down product too, with half the step: what
+// the parts of the hidden values cost does not grow with the rows (layer of 128 experts (2048, 768), top 8, bf16, against one
+// tile: 4 tokens 54.2 against 55.2 us, 16 tokens 123.4 against 125.6, 64 tokens 232 against 235).
+template <int W, int F16>
 struct MoeUnit {
-  static constexpr int kTiles = W == kMoe16 ? 1 : 2;
-  static constexpr float kLift = W == kMoeNvfp4 ? kNvfp4Lift : 1.0f;
+  using GateUp = WeightStep<F16, 1, 8>;
+  using Down = WeightStep<F16, 2, 4>;
+  static constexpr int kTiles = 1, kDownTiles = 2;
+  static constexpr float kLift = 1.0f;
 };
-
-// One step of either kind against NT tiles; `b[j]` is column g of tile j.
-template <int W, int F16, int NT>
-struct MoeStep {
-  static constexpr int MT = MoeUnit<W>::kTiles;
-  using Weights = typename std::conditional<W == kMoe16, WeightStep<W, F16, MT>, WeightStep4<W, MT>>::type;
-  static B200_DEVICE void mma(const Weights& w, float (&acc)[NT][MT][4], const uint16_t* const (&b)[NT], int k0, int K,
-                              uint32_t lane) {
-    if constexpr (W == kMoe16) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) w.mma(acc[j], b[j], k0, K, lane);
-    } else if (k0 + kMoeStep > K || w.general()) {
-      w.template mma<NT, true>(acc, b, k0, K, lane);
-    } else {
-      w.template mma<NT, false>(acc, b, k0, K, lane);
-    }
-  }
+template <>
+struct MoeUnit<kMoeMxfp4, 0> {
+  using GateUp = WeightStep4<kMoeMxfp4, 2, 2>;
+  using Down = WeightStep4<kMoeMxfp4, 2, 2>;
+  static constexpr int kTiles = 2, kDownTiles = 2;
+  static constexpr float kLift = 1.0f;
+};
+template <>
+struct MoeUnit<kMoeNvfp4, 0> {
+  using GateUp = WeightStep4<kMoeNvfp4, 2, 2>;
+  using Down = WeightStep4<kMoeNvfp4, 2, 2>;
+  static constexpr int kTiles = 2, kDownTiles = 2;
+  static constexpr float kLift = kNvfp4Lift;
 };
 
 B200_DEVICE float silu(float v) { return __fdiv_rn(v, 1.0f + expf(-v)); }
 
-// The tokens of an expert ride on the MMA's N in the order of its pairs, two n-tiles at a time (more would
-// need more registers than the weights leave). Columns beyond the last token repeat it and are not used.
+// The tokens of an expert ride on the MMA's N in the order of its pairs, in the gate/up product two n-tiles at a time (more
+// would need more registers than the weights leave). Columns beyond the last token repeat it and are not used.
 
 // ------------------------------------------------------------------------------------- gate and up
 // Unit: 8 intermediate columns per MMA tile of one chosen expert = 8 gate rows and the 8 up rows beside them, so that
@@ -651,9 +844,10 @@ struct UnitCursor {
 
 template <int W, int F16>
 struct GateUp {
-  static constexpr int MT = MoeUnit<W>::kTiles;
+  static constexpr int MT = MoeUnit<W, F16>::kTiles;
   static constexpr int kCols = 8 * MT;
-  using Weights = typename MoeStep<W, F16, 1>::Weights;
+  using Weights = typename MoeUnit<W, F16>::GateUp;
+  static constexpr int kStep = Weights::kStep;
   const MoeArgs& args;
   const RouteTables& r;
   uint32_t lane;
@@ -676,7 +870,7 @@ struct GateUp {
       b[j] = args.x + static_cast<long long>(r.tokens[first_pair + c]) * args.H;
     }
     float acc[NT][MT][4] = {};
-    MoeStep<W, F16, NT>::mma(w, acc, b, k0, args.H, lane);
+    w.mma_tokens(acc, b, k0, args.H, lane);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -699,9 +893,9 @@ struct GateUp {
   B200_DEVICE void run(float4* red, int stride, const UnitCursor& unit, const UnitCursor& next) {
     const int tokens = r.size[unit.index], first_pair = r.first[unit.index];
     const int n_tiles = (tokens + 7) / 8;
-    const int own = warp * kMoeStep;
+    const int own = warp * kStep;
     float4* mine = red + warp * stride;
-    for (int k0 = own; k0 - own < args.H; k0 += kMoeWarps * kMoeStep) {
+    for (int k0 = own; k0 - own < args.H; k0 += kMoeWarps * kStep) {
       if (k0 < args.H) {
         int j = 0;
         for (; j + 1 < n_tiles; j += 2) tiles<2>(mine, first_pair, tokens, j, k0, k0 == own);
@@ -709,7 +903,7 @@ struct GateUp {
       } else if (k0 == own) {
         for (int i = 0; i < n_tiles * MT; ++i) mine[i * 32 + lane] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       }
-      const int k_next = k0 + kMoeWarps * kMoeStep;
+      const int k_next = k0 + kMoeWarps * kStep;
       if (k_next - own < args.H) {
         if (k_next < args.H) load(unit, k_next);
       } else if (next.index < experts && own < args.H) {
@@ -730,12 +924,8 @@ struct GateUp {
         up += at[p * stride * 4 + 2];
       }
       const float h = r.weights[first_pair + c] * (silu(gate * args.lift1) * (up * args.lift1));
-      uint16_t* to = args.h + static_cast<long long>(r.pairs[first_pair + c]) * 2 * args.I + row;
-      const uint16_t nearest = round16<F16>(h);
-      to[0] = nearest;
-      // (beyond the type's range h becomes infinite, as it would in one part, and not the NaN of inf - inf)
-      const float rest = h - widen16<F16>(nearest);
-      to[args.I] = round16<F16>(isinf(rest) || isinf(h) ? 0.0f : rest);
+      uint16_t* to = args.h + static_cast<long long>(r.pairs[first_pair + c]) * 2 * args.I + MoeUnit<W, F16>::Down::hidden_place(row);
+      HiddenParts<F16>::store(h, to, to + args.I);
     }
   }
 };
@@ -754,8 +944,8 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __gri
   constexpr int kCols = GateUp<W, F16>::kCols;
   extern __shared__ __align__(16) uint8_t smem[];
   float4* red = reinterpret_cast<float4*>(smem);
-  const int stride = gate_up_stride(MoeUnit<W>::kTiles, args.T);
-  const int buffers = gate_up_buffers(MoeUnit<W>::kTiles, args.T);
+  const int stride = gate_up_stride(MoeUnit<W, F16>::kTiles, args.T);
+  const int buffers = gate_up_buffers(MoeUnit<W, F16>::kTiles, args.T);
   const RouteTables r = route_tables_at(smem + buffers * kMoeWarps * stride * 16, args);
   const int strips = (args.I + kCols - 1) / kCols;
   const int by_index = static_cast<int>(gridDim.x) / strips, by_strip = static_cast<int>(gridDim.x) % strips;
@@ -765,7 +955,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __gri
   ptx::grid_launch_dependents();
   build_route_tables(r, args);
   GateUp<W, F16> g{args, r, ptx::lane_id(), static_cast<int>(threadIdx.x) / 32, *r.count, {}};
-  if (unit.index < g.experts && g.warp * kMoeStep < args.H) g.load(unit, g.warp * kMoeStep);
+  if (unit.index < g.experts && g.warp * GateUp<W, F16>::kStep < args.H) g.load(unit, g.warp * GateUp<W, F16>::kStep);
   for (int turn = 0; unit.index < g.experts; turn ^= buffers - 1) {
     UnitCursor next = unit;
     next.advance(strips, by_index, by_strip);
@@ -783,9 +973,10 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_gate_up_kernel(const __gri
 // tiles of eight: 172 us against 71 for 64 tokens, 128 experts, 2048 x 768).
 template <int W, int F16>
 struct Down {
-  static constexpr int MT = MoeUnit<W>::kTiles;
+  static constexpr int MT = MoeUnit<W, F16>::kDownTiles;
   static constexpr int kPitch = MT * 16 + 1;  // floats between tokens
-  using Weights = typename MoeStep<W, F16, 1>::Weights;
+  using Weights = typename MoeUnit<W, F16>::Down;
+  static constexpr int kStep = Weights::kStep;
   const MoeArgs& args;
   const RouteTables& r;
   uint32_t lane;
@@ -795,45 +986,58 @@ struct Down {
   B200_DEVICE void load(int s) {
     const int e = r.list[s / steps];
     const int H = args.H, first = r0 + static_cast<int>(lane >> 2);
-    w.load(args.w2, s % steps * kMoeStep, args.I, lane, [=](int m, int half) {
+    w.load(args.w2, s % steps * kStep, args.I, lane, [=](int m, int half) {
       const int row = first + m * 16 + half * 8;
       return row < H ? e * H + row : -1;
     });
   }
 
-  // The loaded step against tiles [j0, j0 + NT) of the expert's tokens, on top of the tokens' sums.
-  template <int NT>
-  B200_DEVICE void tiles(float* sums, int first_pair, int tokens, int j0, int k0) {
-    const uint16_t* b[NT];
+  // The loaded step against the expert's tokens from c0 on, as many as the columns take, on top of the tokens' sums.
+  template <typename Hidden>
+  B200_DEVICE void tile(float* sums, int first_pair, int tokens, int c0, int k0) {
+    constexpr int P = HiddenParts<F16>::kParts, kWidth = 8 / Hidden::kTokens;
+    const int column = static_cast<int>(lane >> 2);
+    const int token = min(c0 + column / kWidth, tokens - 1);
+    const Hidden columns(args.h + static_cast<long long>(r.pairs[first_pair + token]) * 2 * args.I, args.I, column);
+    float acc[Hidden::kSums][MT][4] = {};
+    w.mma_hidden(acc, columns, k0, args.I, lane);
+    // A lane holds columns 2 (lane % 4) and the next one, of rows lane / 4 + 8 m.
+    const auto add = [&](int c, auto part) {
+      const bool live = c < tokens;
+      float* to = sums + r.tokens[first_pair + (live ? c : 0)] * kPitch + (lane >> 2);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      // columns 2 c and 2 c + 1 of a tile are the two parts of its token c
-      const int column = static_cast<int>(lane >> 2);
-      const int c = min((j0 + j) * 4 + column / 2, tokens - 1);
-      b[j] = args.h + (static_cast<long long>(r.pairs[first_pair + c]) * 2 + column % 2) * args.I;
-    }
-    float acc[NT][MT][4] = {};
-    MoeStep<W, F16, NT>::mma(w, acc, b, k0, args.I, lane);
+      for (int m = 0; m < 2 * MT; ++m) {
+        float v[P];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int c = (j0 + j) * 4 + static_cast<int>(lane & 3u);
-      if (c < tokens) {
-        float* to = sums + r.tokens[first_pair + c] * kPitch + (lane >> 2);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          to[m * 16] += acc[j][m][0] + acc[j][m][1];
-          to[m * 16 + 8] += acc[j][m][2] + acc[j][m][3];
-        }
+        for (int p = 0; p < P; ++p) v[p] = part(p, m);
+        if (live) to[m * 8] += join_parts<F16>(v);
       }
+    };
+    const int quad = static_cast<int>(lane & 3u);
+    if constexpr (Hidden::kSums == P) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        add(c0 + quad * 2 + n, [&](int p, int m) { return acc[p][m / 2][m % 2 * 2 + n]; });
+      }
+    } else if constexpr (P == 2) {
+      add(c0 + quad, [&](int p, int m) { return acc[0][m / 2][m % 2 * 2 + p]; });
+    } else {
+      // the third part is the next lane's
+      add((quad & 1) ? tokens : c0 + quad / 2, [&](int p, int m) {
+        return p < 2 ? acc[0][m / 2][m % 2 * 2 + p] : __shfl_xor_sync(0xFFFFFFFFu, acc[0][m / 2][m % 2 * 2], 1);
+      });
     }
   }
 
   B200_DEVICE void run(float* sums, int s, int next, int total) {
-    const int tokens = r.size[s / steps], first_pair = r.first[s / steps];
-    const int n_tiles = (tokens + 3) / 4, k0 = s % steps * kMoeStep;
-    int j = 0;
-    for (; j + 1 < n_tiles; j += 2) tiles<2>(sums, first_pair, tokens, j, k0);
-    if (j < n_tiles) tiles<1>(sums, first_pair, tokens, j, k0);
+    const int tokens = r.size[s / steps], first_pair = r.first[s / steps], k0 = s % steps * kStep;
+    using Few = HiddenColumns<F16>;
+    using Many = HiddenSums<F16>;
+    if (tokens <= Few::kTokens) {
+      tile<Few>(sums, first_pair, tokens, 0, k0);
+    } else {
+      for (int c = 0; c < tokens; c += Many::kTokens) tile<Many>(sums, first_pair, tokens, c, k0);
+    }
     if (next < total) load(next);
     __syncwarp();  // the next step's lanes may hold other tokens
   }
@@ -848,7 +1052,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_c
   const RouteTables r = route_tables_at(smem + (kMoeWarps * per_warp * 4 + 15) / 16 * 16, args);
   const int warp = static_cast<int>(threadIdx.x) / 32;
   const int rank = split > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
-  D d{args, r, ptx::lane_id(), static_cast<int>(blockIdx.x) / split * 16 * D::MT, (args.I + kMoeStep - 1) / kMoeStep, {}};
+  D d{args, r, ptx::lane_id(), static_cast<int>(blockIdx.x) / split * 16 * D::MT, (args.I + D::kStep - 1) / D::kStep, {}};
   for (int i = static_cast<int>(threadIdx.x); i < kMoeWarps * per_warp; i += kMoeThreads) sums[i] = 0.0f;
   // The routing and the weights are there already: every CTA of the gate/up kernel had waited for the router before this
   // kernel was allowed to start. So the first step's weights are under way while that kernel finishes; its
