@@ -123,7 +123,8 @@ B200_DEVICE uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
 // bf16: the fp32 number, rounded to 22 significant bits: its upper half, and the next two groups of 7 bits, m1 below m2. With
 // E = +-2^e, sign and exponent alone, the parts are the upper half itself, E * m1 / 128 and E * m2 / 128: each
 // exact in bf16 and two or three instructions for two elements (E | m is E + E m / 128).
-// fp16: the nearest fp16 number, and the nearest one of what that leaves.
+// fp16: the nearest fp16 number, and the nearest one of 2^11 times what that leaves, which is at most 2^15 (half a step of
+// the largest numbers) and, unscaled, would be subnormal for hidden values below a quarter. 22 bits from 2^-14 on, 2^-36 below.
 template <int F16>
 struct HiddenParts;
 
@@ -156,11 +157,11 @@ struct HiddenParts<0> {
 template <>
 struct HiddenParts<1> {
   static constexpr int kParts = 2;
-  static B200_DEVICE float factor(int) { return 1.0f; }
+  static B200_DEVICE float factor(int p) { return p == 0 ? 1.0f : 0.00048828125f; }  // 1, 2^-11
   static B200_DEVICE void store(float h, uint16_t* first, uint16_t* second) {
     *first = round16<1>(h);
     // (beyond the type's range h becomes infinite, as it would in one part, and not the NaN of inf - inf)
-    const float rest = h - widen16<1>(*first);
+    const float rest = (h - widen16<1>(*first)) * 2048.0f;
     *second = round16<1>(isinf(rest) || isinf(h) ? 0.0f : rest);
   }
   static B200_DEVICE void all(uint32_t (&part)[kParts], uint32_t first, uint32_t second) {

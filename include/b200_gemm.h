@@ -309,7 +309,7 @@ int b200_gemm_mx(int format, int f16, int M, int N, int K, const void* A, const 
  *   S[t]    = the top_k largest l[t, .], ties to the lower index, -inf never chosen, NaN before all others
  *   p[t, e] = exp(l[t, e]) / sum of exp(l[t, .]) over S[t] (renormalize) or over all experts
  *   h[t, e] = p[t, e] silu(W1[e, 0 : I] X[t]) (W1[e, I : 2 I] X[t])      fp32, of which W2 meets 22 bits (bf16 X), or the
- *             nearest fp16 number and that of the rest (fp16 X: infinite beyond 65504)
+ *             nearest fp16 number and that of 2^11 times the rest (fp16 X: infinite beyond 65504)
  *   out[t]  = sum over S[t] of W2[e] h[t, e]              fp32 sum, rounded once; 0 when S[t] is empty
  * X [T, H], router [E, H], W1 [E, 2 I, H] (gate rows, then up rows), W2 [E, H, I], out [T, H]: bf16, or fp16
  * with f16 = 1, contiguous, X and weights on 16 bytes. weight_format B200_MXFP4 / B200_NVFP4: W1 and W2

@@ -81,3 +81,29 @@ def test_infinite_and_nan_hidden_values(kind):
     x[2, 3] = math.nan
     out = layer(x.cuda(), torch.ones(8, 24), kind)
     assert (out[0] == math.inf).all() and (out[1] == -math.inf).all() and out[2].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 7])
+@pytest.mark.parametrize("size", [2.0 ** -8, 2.0 ** -12, 2.0 ** -15])
+def test_small_fp16_hidden_values(size, T):
+    """Small hidden values (a routing weight of a hundredth is enough) under large down weights: the rest behind the
+    nearest fp16 number is far below fp16's smallest one.
+
+    Off by: 2^-20 as above, and 2^-36 where that rest is subnormal; 1024 times that, and half a step of the output."""
+    n = 64
+    gen = torch.Generator().manual_seed(T)
+    gate = (torch.rand(T, n, generator=gen) * 4 + 1).to(FP16)
+    up = ((torch.rand(T, n, generator=gen) + 0.5) * size).to(FP16)
+    h = silu(gate.double()) * up.double()
+    near = (h / 32).to(FP16)                                   # 32 times it is taken off, so that the rest shows
+    gates = torch.stack([gate, torch.full_like(gate, 32.0)], 2)
+    ups = torch.stack([up, near], 2)
+    down = torch.zeros(n, 2 * n)
+    for r in range(n):
+        down[r, 2 * r], down[r, 2 * r + 1] = 1024, -1024
+    out = layer(torch.cat([gates.view(T, -1), ups.view(T, -1)], 1).cuda(), down, "fp16").double().cpu()
+    want = 1024 * (h - 32 * near.double())
+    bound = 1024 * (2.0 ** -20 * h + 2.0 ** -36) + 2.0 ** -11 * want.abs() + 2.0 ** -25
+    off = (out - want).abs()
+    assert (off <= bound).all(), f"{(off > bound).sum()} of {off.numel()} outside, up to {(off / bound).max():.2g} times the bound"
