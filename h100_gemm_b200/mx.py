@@ -106,6 +106,10 @@ class MxTensor:
         self._scales_ptr = self._data_ptr + at
         return self
 
+    def __reduce__(self):
+        """Copies and pickles hold the tensors; the addresses that kernels get are theirs, not this object's."""
+        return type(self), (self.data, self.scales, self.rows, self.cols, self.format, self.tensor_scale)
+
     @property
     def data(self):
         if self._data is None:

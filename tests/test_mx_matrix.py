@@ -1,0 +1,74 @@
+"""MxTensor as a Python object: copies, pickles, sizes and scales at the ends of their ranges."""
+import copy
+import io
+import pickle
+
+import pytest
+import torch
+
+import h100_gemm_b200 as g
+from h100_gemm_b200 import api
+
+FORMATS = ["mxfp4", "nvfp4"]
+
+
+def saved_and_loaded(q):
+    file = io.BytesIO()
+    torch.save({"weight": q}, file)
+    file.seek(0)
+    return torch.load(file, weights_only=False)["weight"]
+
+
+COPIES = {"copy": copy.copy, "deepcopy": copy.deepcopy, "pickle": lambda q: pickle.loads(pickle.dumps(q)),
+          "save": saved_and_loaded, "nested": lambda q: copy.deepcopy({"a": [q], "b": q})["b"]}
+
+
+def cpu_matrix(rows, cols, fmt, one_allocation):
+    if one_allocation:
+        q = g.MxTensor._empty(rows, cols, fmt, 2.0 if fmt == "nvfp4" else 1.0, torch.device("cpu"))
+    else:
+        lib = api.library()
+        q = g.MxTensor(torch.zeros(rows, lib.b200_mx_data_bytes(1, cols), dtype=torch.uint8),
+                       torch.zeros(lib.b200_mx_scale_bytes({"mxfp4": 0, "nvfp4": 1}[fmt], rows, cols), dtype=torch.uint8),
+                       rows, cols, fmt, 2.0 if fmt == "nvfp4" else 1.0)
+    q.data.copy_(torch.randint(0, 256, q.data.shape, dtype=torch.uint8))
+    q.scales.copy_(torch.randint(0, 127, q.scales.shape, dtype=torch.uint8))
+    return q
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("one_allocation", [True, False])
+@pytest.mark.parametrize("how", COPIES)
+def test_copies_point_at_their_own_memory(how, one_allocation, fmt):
+    q = cpu_matrix(70, 300, fmt, one_allocation)
+    c = COPIES[how](q)
+    assert (c.rows, c.cols, c.format, c.tensor_scale, c.device) == (q.rows, q.cols, q.format, q.tensor_scale, q.device)
+    assert torch.equal(c.data, q.data) and torch.equal(c.scales, q.scales)
+    for m in (q, c):
+        assert m._data_ptr == m.data.data_ptr() and m._scales_ptr == m.scales.data_ptr()
+        assert m._data_ptr % 16 == 0 and m._scales_ptr % 16 == 0
+    if how == "copy":
+        assert c._data_ptr == q._data_ptr                 # a shallow copy shares its tensors, as that of any object does
+    else:
+        before = q.data.clone()
+        c.data.zero_()
+        assert c._data_ptr != q._data_ptr and torch.equal(q.data, before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "save"])
+def test_copies_multiply_with_their_own_values(how, fmt):
+    gen = torch.Generator().manual_seed(1)
+    w = torch.randn(200, 512, generator=gen).bfloat16().cuda()
+    x = g.quantize_mx(torch.randn(5, 512, generator=gen).bfloat16().cuda(), fmt)
+    q = g.quantize_mx(w, fmt)
+    want = g.gemm_mx(x, q)
+    c = COPIES[how](q)
+    q.data.zero_()                                        # the original's memory is not what the copy reads
+    assert not g.gemm_mx(x, q).any()
+    del q
+    assert torch.equal(g.gemm_mx(x, c), want)
+    c.data.copy_(g.quantize_mx(-w, fmt).data)             # what is written into a copy is what it multiplies with
+    assert torch.equal(g.gemm_mx(x, c), -want)
+    assert torch.equal(g.dequantize_mx(c), g.dequantize_mx(g.quantize_mx(-w, fmt)))
