@@ -17,6 +17,8 @@ blocks have to run along the contraction::
 from __future__ import annotations
 
 import contextlib
+import ctypes
+import math
 
 from . import api
 from .api import STATUS_INVALID_ARG, GemmError
@@ -39,6 +41,7 @@ torch = _Torch(globals())
 
 FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
+FP32_MIN, FP32_MAX = 2.0 ** -126, 2.0 ** 128 - 2.0 ** 104  # its normal numbers
 _GROUPS = {"mxfp4": 2, "nvfp4": 4}  # 512-byte scale groups of a 128 x 256 tile
 
 
@@ -74,8 +77,8 @@ class MxTensor:
         _format(format)
         if rows <= 0 or cols <= 0:
             raise _invalid("rows and cols must be positive")
-        if not 0 < tensor_scale < 3.4e38:
-            raise _invalid("tensor_scale must be positive and finite in fp32")
+        if not FP32_MIN <= tensor_scale < 3.4e38:
+            raise _invalid("tensor_scale must be a positive normal number in fp32")
         if format == "mxfp4" and tensor_scale != 1.0:
             raise _invalid("mxfp4 has no tensor scale (it must be 1)")
         pointers = []
@@ -299,9 +302,18 @@ def _launch_dequantize(q, dtype, f16, out, ld, handle):
     return out
 
 
+def _unusual_factor(factor: float, alpha: float) -> None:
+    """Raises where alpha times the tensor scales is not what fp32 can hold. (An alpha of zero, an infinite or a NaN one
+    mean what they say, and a small power of two is exact.)"""
+    if alpha == 0 or not math.isfinite(alpha) or (abs(factor) < 1 and ctypes.c_float(factor).value == factor):
+        return
+    raise _invalid(f"alpha times the tensor scales of a and b is {factor}, outside fp32's range: leave a power of two of it to the caller")
+
+
 def gemm_mx(a: MxTensor, b: MxTensor, out=None, alpha: float = 1.0, beta: float = 0.0, dtype=None, stream=None):
     """out[M, N] = (a[M, K] @ b[N, K]^T) * alpha + beta for two 4-bit matrices of one format, tensor scales
-    applied; bf16 (default) or fp16 output, fp32 accumulation."""
+    applied (their product with alpha has to be within fp32's range); bf16 (default) or fp16 output, fp32
+    accumulation."""
     if not isinstance(a, MxTensor) or not isinstance(b, MxTensor):
         raise _invalid(f"a and b must be MxTensors, got {type(a).__name__} and {type(b).__name__}")
     dtype = dtype or (out.dtype if out is not None else torch.bfloat16)
@@ -310,6 +322,9 @@ def gemm_mx(a: MxTensor, b: MxTensor, out=None, alpha: float = 1.0, beta: float 
         raise _invalid(f"a is {a.format}, b is {b.format}")
     if a.cols != b.cols:
         raise _invalid("a and b disagree on K")
+    factor = alpha * a.tensor_scale * b.tensor_scale
+    if not FP32_MIN <= abs(factor) <= FP32_MAX:
+        _unusual_factor(factor, alpha)
     device = a.device
     _require_cuda(device, "a")
     _require_cuda(b.device, "b", device)
@@ -318,16 +333,16 @@ def gemm_mx(a: MxTensor, b: MxTensor, out=None, alpha: float = 1.0, beta: float 
 
     handle = _current(device, stream)
     if handle is not False:
-        return _launch_gemm(a, b, dtype, f16, out, alpha, beta, handle)
+        return _launch_gemm(a, b, dtype, f16, out, factor, beta, handle)
     with _elsewhere(device, stream) as handle:
-        return _launch_gemm(a, b, dtype, f16, out, alpha, beta, handle)
+        return _launch_gemm(a, b, dtype, f16, out, factor, beta, handle)
 
 
-def _launch_gemm(a, b, dtype, f16, out, alpha, beta, handle):
+def _launch_gemm(a, b, dtype, f16, out, factor, beta, handle):
     if out is None:
         out = torch.empty(a.rows, b.rows, dtype=dtype, device=a.device)
     rc = api.library().b200_gemm_mx(FORMATS[a.format], f16, a.rows, b.rows, a.cols, a._data_ptr, a._scales_ptr, b._data_ptr,
-                                    b._scales_ptr, out.data_ptr(), alpha * a.tensor_scale * b.tensor_scale, beta, handle)
+                                    b._scales_ptr, out.data_ptr(), factor, beta, handle)
     if rc:
         api._check(rc)
     return out

@@ -72,3 +72,39 @@ def test_copies_multiply_with_their_own_values(how, fmt):
     c.data.copy_(g.quantize_mx(-w, fmt).data)             # what is written into a copy is what it multiplies with
     assert torch.equal(g.gemm_mx(x, c), -want)
     assert torch.equal(g.dequantize_mx(c), g.dequantize_mx(g.quantize_mx(-w, fmt)))
+
+
+def test_tensor_scales_that_fp32_cannot_hold():
+    data, scales = torch.zeros(4, 32, dtype=torch.uint8), torch.zeros(2048, dtype=torch.uint8)
+    for bad in (0.0, -1.0, 1e-50, 2.0 ** -130, 3.5e38, float("inf"), float("nan")):
+        with pytest.raises(g.GemmError, match="tensor_scale"):
+            g.MxTensor(data, scales, 4, 64, "nvfp4", bad)
+    matrix = lambda ts: g.MxTensor(data, scales, 4, 64, "nvfp4", ts)  # noqa: E731
+    # two legal scales whose product is not a number of fp32, or loses its bits
+    for a, b, alpha in ((2.0 ** 64, 2.0 ** 64, 1.0), (1e30, 1e30, 1.0), (2.0 ** 64, 1.0, 2.0 ** 64), (1e-25, 1e-25, 1.0),
+                        (1e-20, 1e-20, 0.3), (2.0 ** 64, 2.0 ** 64, -1.0)):
+        with pytest.raises(g.GemmError, match="outside fp32's range"):
+            g.gemm_mx(matrix(a), matrix(b), alpha=alpha)
+    # the same undone by alpha, powers of two that are exact, and what an alpha means by itself: refused for the device alone
+    for a, b, alpha in ((2.0 ** 64, 2.0 ** 64, 2.0 ** -100), (2.0 ** -64, 2.0 ** -64, 1.0), (2.0 ** 64, 2.0 ** 64, 0.0),
+                        (1e-25, 1e-25, 1e20), (1.0, 1.0, float("inf")), (1.0, 1.0, float("nan"))):
+        with pytest.raises(g.GemmError, match="CUDA tensor"):
+            g.gemm_mx(matrix(a), matrix(b), alpha=alpha)
+
+
+@pytest.mark.gpu
+def test_products_under_far_tensor_scales():
+    """Scales of 2^64 and 2^-64 on both sides, brought back by alpha: the same bits, and zeros stay zeros."""
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(300, 512, generator=gen)
+    x[3] = 0
+    x = x.bfloat16().cuda()
+    base = g.quantize_mx(x, "nvfp4")
+    want = g.gemm_mx(base, base)
+    assert not want[3].any() and want.isfinite().all()
+    for e in (64, -64):
+        q = g.quantize_mx((x.double() * 2.0 ** e).bfloat16(), "nvfp4", tensor_scale=2.0 ** e)
+        assert torch.equal(g.gemm_mx(q, q, alpha=2.0 ** (-2 * e)), want)
+        assert torch.equal(g.gemm_mx(q, base, alpha=2.0 ** -e), want)
+    q = g.quantize_mx((x.double() * 2.0 ** -50).bfloat16(), "nvfp4", tensor_scale=2.0 ** -50)
+    assert torch.equal(g.gemm_mx(q, q).double(), want.double() * 2.0 ** -100)
