@@ -21,6 +21,9 @@ bool sizes_ok(int T, int E, int k, int H, int I) {
          I >= 8 && H % 8 == 0 && I % 8 == 0 && H <= (1 << 20) && I <= (1 << 20);
 }
 
+// What b200_mx_dequantize takes.
+bool weights_scale_ok(int format, float t) { return t > 0.0f && t <= 3.4e38f && (format == B200_NVFP4 || t == 1.0f); }
+
 struct Launch {
   cudaLaunchConfig_t config = {};
   cudaLaunchAttribute attr[2];
@@ -101,6 +104,9 @@ int b200_moe_layer(int f16, int T, int E, int top_k, int H, int I, const void* X
   if (four_bit && f16) return B200_ERR_INVALID_ARG;
   if (X == nullptr || router == nullptr || W1 == nullptr || W2 == nullptr || out == nullptr) return B200_ERR_INVALID_ARG;
   if (four_bit && (W1_scales == nullptr || W2_scales == nullptr)) return B200_ERR_INVALID_ARG;
+  if (four_bit && !(weights_scale_ok(weight_format, W1_tensor_scale) && weights_scale_ok(weight_format, W2_tensor_scale))) {
+    return B200_ERR_INVALID_ARG;
+  }
   if (!aligned16(X) || !aligned16(router) || !aligned16(W1) || !aligned16(W2) || !aligned16(W1_scales) ||
       !aligned16(W2_scales) || (reinterpret_cast<uintptr_t>(out) & 1u) || (reinterpret_cast<uintptr_t>(bias) & 3u) ||
       (reinterpret_cast<uintptr_t>(ids) & 3u) || (reinterpret_cast<uintptr_t>(weights) & 3u)) {
@@ -131,9 +137,8 @@ int b200_moe_layer(int f16, int T, int E, int top_k, int H, int I, const void* X
   args.w2.scales = static_cast<const uint8_t*>(W2_scales);
   args.w2.pitch = four_bit ? mx_pitch(I) : 2ll * I;
   args.w2.col_tiles = mx_col_tiles(I);
-  const float lift = weight_format == B200_NVFP4 ? MoeUnit<kMoeNvfp4, 0>::kLift : 1.0f;
-  args.lift1 = four_bit ? lift * W1_tensor_scale : 1.0f;
-  args.lift2 = four_bit ? lift * W2_tensor_scale : 1.0f;
+  args.scale1 = four_bit ? W1_tensor_scale : 1.0f;
+  args.scale2 = four_bit ? W2_tensor_scale : 1.0f;
   args.h = reinterpret_cast<uint16_t*>(ws);
   args.ids = ids != nullptr ? ids : reinterpret_cast<int*>(ws + h_bytes(T, top_k, I));
   args.weights = weights != nullptr ? weights : reinterpret_cast<float*>(ws + h_bytes(T, top_k, I) + pair_bytes(T, top_k));

@@ -313,7 +313,8 @@ int b200_gemm_mx(int format, int f16, int M, int N, int K, const void* A, const 
  *   out[t]  = sum over S[t] of W2[e] h[t, e]              fp32 sum, rounded once; 0 when S[t] is empty
  * X [T, H], router [E, H], W1 [E, 2 I, H] (gate rows, then up rows), W2 [E, H, I], out [T, H]: bf16, or fp16
  * with f16 = 1, contiguous, X and weights on 16 bytes. weight_format B200_MXFP4 / B200_NVFP4: W1 and W2
- * are 4-bit matrices of E * 2 I and E * H rows in the layout above, with their tensor scales (bf16 only).
+ * are 4-bit matrices of E * 2 I and E * H rows in the layout above, with their tensor scales as b200_mx_dequantize takes
+ * them (bf16 only).
  * ids [T, top_k] (-1 = no expert) and weights [T, top_k] receive the routing, largest logit first; either may
  * be NULL. Limits: T <= 64, E <= 512, top_k <= 32, H and I multiples of 8. Expert weights have to be
  * finite (a token's zeros meet them). The workspace starts on 256 bytes and is free again when the work on `stream`

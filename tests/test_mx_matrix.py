@@ -92,6 +92,17 @@ def test_tensor_scales_that_fp32_cannot_hold():
             g.gemm_mx(matrix(a), matrix(b), alpha=alpha)
 
 
+def test_tensor_scales_of_expert_weights_are_checked():
+    p = 4096
+    call = lambda fmt, t1, t2: api.library().b200_moe_layer(0, 2, 8, 2, 64, 32, p, p, None, fmt, p, p, t1, p, p, t2, 1, p, None, None,  # noqa: E731
+                                                            None, 0, None)
+    for bad in (0.0, -1.0, float("inf"), float("nan"), -float("inf")):
+        assert call(1, bad, 1.0) == call(1, 1.0, bad) == api.STATUS_INVALID_ARG
+    assert call(0, 2.0, 1.0) == call(0, 1.0, 0.5) == api.STATUS_INVALID_ARG
+    for good in ((0, 1.0, 1.0), (1, 0.37, 3e38)):                    # past the checks: no workspace
+        assert call(*good) == api.STATUS_WORKSPACE
+
+
 @pytest.mark.gpu
 def test_products_under_far_tensor_scales():
     """Scales of 2^64 and 2^-64 on both sides, brought back by alpha: the same bits, and zeros stay zeros."""
@@ -108,3 +119,20 @@ def test_products_under_far_tensor_scales():
         assert torch.equal(g.gemm_mx(q, base, alpha=2.0 ** -e), want)
     q = g.quantize_mx((x.double() * 2.0 ** -50).bfloat16(), "nvfp4", tensor_scale=2.0 ** -50)
     assert torch.equal(g.gemm_mx(q, q).double(), want.double() * 2.0 ** -100)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("e1,e2", [(100, 112), (-100, -100)])
+def test_experts_under_far_tensor_scales(e1, e2):
+    """NVFP4 experts whose tensor scales are far from 1, undone by the tokens (gate and up) or seen in the result."""
+    T, E, k, H, I = 3, 4, 2, 64, 48
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(T, H, generator=gen).bfloat16().cuda()
+    router = torch.zeros(E, H, dtype=torch.bfloat16, device="cuda")
+    w1 = g.quantize_mx(torch.randn(E * 2 * I, H, generator=gen).bfloat16().cuda(), "nvfp4")
+    w2 = g.quantize_mx(torch.randn(E * H, I, generator=gen).bfloat16().cuda(), "nvfp4")
+    want = g.moe_layer(x, router, w1, w2, k)
+    far = lambda q, e: g.MxTensor(q.data, q.scales, q.rows, q.cols, "nvfp4", 2.0 ** e)  # noqa: E731
+    undone = (x.double() * 2.0 ** -e1).bfloat16()
+    assert torch.equal(g.moe_layer(undone, router, far(w1, e1), w2, k), want)
+    assert torch.equal(g.moe_layer(x, router, w1, far(w2, e2), k).double(), want.double() * 2.0 ** e2)
