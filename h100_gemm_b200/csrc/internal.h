@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cstdint>
+#include <cstdlib>
 
 #include "../../include/b200_gemm.h"
 
@@ -36,6 +38,32 @@ int cuda_failed(int error);
       return ::b200::cuda_failed(static_cast<int>(e__));                       \
     }                                                                          \
   } while (0)
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Whether a launch may overlap the kernel before it in the stream (B200_GEMM_NO_PDL=1 turns that off).
+inline int programmatic_launch() { return std::getenv("B200_GEMM_NO_PDL") ? 0 : 1; }
+
+// A launch of a one-dimensional grid in stream order, in clusters, with the set-up overlapping the kernel before it: the
+// kernel waits for that one to complete before it touches what it may write or still read.
+struct Launch {
+  cudaLaunchConfig_t config = {};
+  cudaLaunchAttribute attr[2];
+  Launch(long long grid, int threads, size_t smem, cudaStream_t stream, int cluster = 1) {
+    config.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+    config.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = programmatic_launch();
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    config.attrs = attr;
+    config.numAttrs = cluster > 1 ? 2 : 1;
+  }
+};
 
 // Lets a kernel use all of the device's shared memory; asked for once per device (`done`: the kernel's own flags).
 template <typename Kernel>

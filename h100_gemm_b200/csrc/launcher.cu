@@ -1071,7 +1071,7 @@ int run_gemm(int batch, int M, int N, int K, const void* A, long long strideA, c
   // Let this kernel's set-up overlap the tail of whatever runs before it in the stream; the
   // kernel itself waits (griddepcontrol.wait) before it touches global memory.
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = std::getenv("B200_GEMM_NO_PDL") ? 0 : 1;
+  attr[1].val.programmaticStreamSerializationAllowed = b200::programmatic_launch();
   lc.attrs = attr;
   lc.numAttrs = 2;
   // (the tracing build exists for bf16 only; fp16 launches are never traced)

@@ -8,8 +8,6 @@ namespace {
 
 using namespace b200;
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 size_t round_up(size_t x) { return (x + 255) / 256 * 256; }
 
 // Workspace: [h][ids][weights]
@@ -23,25 +21,6 @@ bool sizes_ok(int T, int E, int k, int H, int I) {
 
 // What b200_mx_dequantize takes.
 bool weights_scale_ok(int format, float t) { return t > 0.0f && t <= 3.4e38f && (format == B200_NVFP4 || t == 1.0f); }
-
-struct Launch {
-  cudaLaunchConfig_t config = {};
-  cudaLaunchAttribute attr[2];
-  Launch(int grid, int threads, int smem, cudaStream_t stream, int cluster) {
-    config.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-    config.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
-    config.dynamicSmemBytes = static_cast<size_t>(smem);
-    config.stream = stream;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    config.attrs = attr;
-    config.numAttrs = cluster > 1 ? 2 : 1;
-  }
-};
 
 template <int W, int F16>
 int launch_all(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) {

@@ -9,8 +9,6 @@ namespace {
 
 using namespace b200;
 
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 bool format_known(int format) { return format == B200_MXFP4 || format == B200_NVFP4; }
 
 // Powers of two within fp32's comfortable range, so that dividing by one is exact.
@@ -21,27 +19,6 @@ bool tensor_scale_ok(int format, float t) {
   if ((bits & 0x807FFFFFu) != 0 || exponent < -64 || exponent > 64) return false;
   return format == B200_NVFP4 || t == 1.0f;
 }
-
-// A launch in stream order with the set-up overlapping the kernel before it (every kernel here
-// waits for that kernel to complete before it touches global memory).
-struct Launch {
-  cudaLaunchConfig_t config = {};
-  cudaLaunchAttribute attr[2];
-  Launch(long long grid, int threads, size_t smem, cudaStream_t stream, int cluster = 1) {
-    config.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-    config.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
-    config.dynamicSmemBytes = smem;
-    config.stream = stream;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-    attr[1].val.clusterDim.y = 1;
-    attr[1].val.clusterDim.z = 1;
-    config.attrs = attr;
-    config.numAttrs = cluster > 1 ? 2 : 1;
-  }
-};
 
 template <int FMT, int F16, int ROW, int COL>
 int launch_quantize(const QuantArgs& args, bool vec, long long grid, cudaStream_t stream) {

@@ -95,7 +95,7 @@ typedef struct b200_gemm_cfg {
  * Asynchronous on `stream`; no host synchronisation, no allocation. The kernel is launched with
  * programmatic stream serialization: its set-up may overlap the tail of the kernel before it in
  * the stream, and it waits for that kernel to complete before it reads or writes global memory
- * (environment variable B200_GEMM_NO_PDL=1 turns this off). */
+ * (environment variable B200_GEMM_NO_PDL=1 turns this off, for all kernels of the library). */
 int b200_gemm_bf16(int M, int N, int K, const void* A, const void* B, void* C, float alpha,
                    float beta, const b200_gemm_cfg* cfg, void* workspace, size_t workspace_bytes,
                    void* stream);
