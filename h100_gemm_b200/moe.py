@@ -7,10 +7,13 @@ from .mx import FORMATS, MxTensor, _current, _elsewhere, _half_type, _invalid, _
 
 torch = _Torch(globals())
 
-MAX_TOKENS, MAX_EXPERTS, MAX_TOP_K = 64, 512, 32
+MAX_TOKENS, MAX_EXPERTS, MAX_TOP_K, MAX_SIZE = 64, 512, 32, 2 ** 20
 
 
 def moe_workspace_bytes(tokens: int, experts: int, top_k: int, hidden: int, inner: int) -> int:
+    """Bytes of ``workspace`` for these sizes; 0 for sizes that moe_layer does not take."""
+    if max(abs(n) for n in (tokens, experts, top_k, hidden, inner)) > MAX_SIZE:
+        return 0  # (the C ABI takes 32-bit numbers)
     return int(api.library().b200_moe_workspace_bytes(tokens, experts, top_k, hidden, inner))
 
 
@@ -63,6 +66,8 @@ def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: 
             raise _invalid(f"w_gate_up must be [{E}, 2 I, {H}] and w_down [{E}, {H}, I]")
     if H % 8 or I % 8 or H == 0 or I == 0:
         raise _invalid("hidden and inner sizes must be multiples of 8")
+    if H > MAX_SIZE or I > MAX_SIZE:
+        raise _invalid(f"hidden and inner sizes of at most {MAX_SIZE}, got {H} and {I}")
     device, dtype = x.device, x.dtype
     _require_cuda(device, "x")
 

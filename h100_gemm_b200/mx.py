@@ -41,6 +41,7 @@ torch = _Torch(globals())
 
 FORMATS = {"mxfp4": 0, "nvfp4": 1}
 BLOCK = {"mxfp4": 32, "nvfp4": 16}
+MAX_SIZE = 2 ** 31 - 1  # rows and columns are 32-bit numbers in the C ABI
 FP32_MIN, FP32_MAX = 2.0 ** -126, 2.0 ** 128 - 2.0 ** 104  # its normal numbers
 _GROUPS = {"mxfp4": 2, "nvfp4": 4}  # 512-byte scale groups of a 128 x 256 tile
 
@@ -77,6 +78,8 @@ class MxTensor:
         _format(format)
         if rows <= 0 or cols <= 0:
             raise _invalid("rows and cols must be positive")
+        if rows > MAX_SIZE or cols > MAX_SIZE:
+            raise _invalid(f"at most {MAX_SIZE} rows and columns, got [{rows}, {cols}]")
         if not FP32_MIN <= tensor_scale < 3.4e38:
             raise _invalid("tensor_scale must be a positive normal number in fp32")
         if format == "mxfp4" and tensor_scale != 1.0:
@@ -220,6 +223,8 @@ def _quantize(x, format, tensor_scale, out, rows: bool, cols: bool, stream):
     f16 = _half_type(x.dtype, "x")
     if x.dim() != 2 or x.numel() == 0:
         raise _invalid("x must be a 2-D tensor with at least one row and one column")
+    if max(x.shape) > MAX_SIZE:
+        raise _invalid(f"at most {MAX_SIZE} rows and columns, got {list(x.shape)}")
     ld = _row_stride(x, "x")
     device = x.device
     _require_cuda(device, "x")

@@ -316,7 +316,7 @@ int b200_gemm_mx(int format, int f16, int M, int N, int K, const void* A, const 
  * are 4-bit matrices of E * 2 I and E * H rows in the layout above, with their tensor scales as b200_mx_dequantize takes
  * them (bf16 only).
  * ids [T, top_k] (-1 = no expert) and weights [T, top_k] receive the routing, largest logit first; either may
- * be NULL. Limits: T <= 64, E <= 512, top_k <= 32, H and I multiples of 8. Expert weights have to be
+ * be NULL. Limits: T <= 64, E <= 512, top_k <= 32, H and I multiples of 8 up to 2^20. Expert weights have to be
  * finite (a token's zeros meet them). The workspace starts on 256 bytes and is free again when the work on `stream`
  * is done; its contents do not matter. Asynchronous, no allocation, results do not depend on timing. */
 #define B200_MOE_16BIT (-1)

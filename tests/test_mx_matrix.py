@@ -136,3 +136,20 @@ def test_experts_under_far_tensor_scales(e1, e2):
     undone = (x.double() * 2.0 ** -e1).bfloat16()
     assert torch.equal(g.moe_layer(undone, router, far(w1, e1), w2, k), want)
     assert torch.equal(g.moe_layer(x, router, w1, far(w2, e2), k).double(), want.double() * 2.0 ** e2)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    """The C ABI's sizes are 32-bit: 2^32 + 5 rows would arrive as 5."""
+    BF16 = torch.bfloat16
+    big = 2 ** 32 + 8
+    meta = lambda *s, dtype=BF16: torch.empty(*s, dtype=dtype, device="meta")  # noqa: E731
+    for x in (meta(big, 1), meta(1, big), meta(2 ** 31, 2)):
+        for call in (g.quantize_mx, g.quantize_mx_both, lambda t: g.quantize_mx(t, transpose=True)):
+            with pytest.raises(g.GemmError, match="rows and columns"):
+                call(x)
+    with pytest.raises(g.GemmError, match="rows and columns"):
+        g.MxTensor(meta(big * 16, dtype=torch.uint8), meta(1, dtype=torch.uint8), big, 32)
+    for H, I in ((big, 8), (8, big), (2 ** 20 + 8, 8)):
+        with pytest.raises(g.GemmError, match="hidden and inner"):
+            g.moe_layer(meta(1, H), meta(2, H), meta(2, 2 * I, H), meta(2, H, I), 1)
+        assert g.moe_workspace_bytes(1, 2, 1, H, I) == 0
