@@ -935,8 +935,8 @@ struct GateUp {
 __host__ __device__ __forceinline__ int moe_token_tiles(int T) { return (T + 7) / 8; }
 // float4 between two warps' sums
 __host__ __device__ __forceinline__ int gate_up_stride(int tiles, int T) { return tiles * moe_token_tiles(T) * 32; }
-// Sums of two units, used in turn, save a barrier per unit; of one where two CTAs per SM have no room for more (4-bit
-// weights and 33 or more tokens: a second buffer left one CTA per SM, 167 against 141 us for 64 tokens of 128 MXFP4 experts).
+// Sums of two units, used in turn, save a barrier per unit; of one where two CTAs per SM have no room for more (4-bit weights and
+// 41 or more tokens: a second buffer left one CTA per SM, the layer 26 us longer for 64 tokens of 128 MXFP4 experts).
 __host__ __device__ __forceinline__ int gate_up_buffers(int tiles, int T) {
   return 2 * kMoeWarps * gate_up_stride(tiles, T) * 16 <= 80 * 1024 ? 2 : 1;
 }
