@@ -124,6 +124,7 @@ MxPlan plan_product(int M, int N, int K, int sms) {
 template <int FMT, int BN, int PAIR, int F16>
 int launch_gemm(const DeviceInfo& dev, const MxProduct& p, const MxPlan& plan, MxGemmArgs args, cudaStream_t stream) {
   using T = MxGemmTraits<FMT, BN, PAIR>;
+  if (!T::kRowMajor && !plan.transposed) return B200_ERR_INVALID_ARG;  // (plan_product never asks for it)
   args.k_tiles = static_cast<int>(mx_col_tiles(p.K));
   args.split = plan.split;
   args.tma_store = !plan.transposed && aligned16(args.C) && args.ldc % 8 == 0 ? 1 : 0;

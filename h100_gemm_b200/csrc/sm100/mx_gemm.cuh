@@ -92,6 +92,8 @@ struct MxGemmTraits {
   static_assert(kNeedCols <= 512, "accumulators and scales exceed tensor memory");
   static_assert(BN % 16 == 0 && BN <= 256 && (!PAIR || BN >= 64), "width of the MMA");
   static_assert(kWBytes % 1024 == 0, "swizzled tiles start on 1024 bytes");
+  // Row-major C comes from the widest tile alone; the narrower ones always write the transposed form.
+  static constexpr bool kRowMajor = BN == 256;
   static constexpr int kBarrierBytes = 512;
   static constexpr int smem_bytes(int stages, int slabs) { return 1024 + stages * kStageBytes + 4 * slabs + kBarrierBytes; }
 };
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
     ptx::prefetch_tensormap(&map_w);
     ptx::prefetch_tensormap(&map_sx);
     ptx::prefetch_tensormap(&map_sw);
-    if (args.tma_store) ptx::prefetch_tensormap(&map_c);
+    if (T::kRowMajor && args.tma_store) ptx::prefetch_tensormap(&map_c);
     for (int s = 0; s < args.stages; ++s) {
       ptx::mbar_init(full_bar(s), 1);
       ptx::mbar_init(empty_bar(s), 1);
@@ -443,7 +445,7 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
       // One 32-column piece of this lane's row, already in the output type, to C.
       auto store = [&](const uint32_t (&p)[kChunk / 2], int c) {
         if (!live || s0 + c >= args.S) return;
-        if (args.transposed) {
+        if (!T::kRowMajor || args.transposed) {
           if (row < args.R) {
 #pragma unroll
             for (int j = 0; j < kChunk; ++j) {
@@ -454,7 +456,7 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
           }
           return;
         }
-        if constexpr (BN >= 64) {
+        if constexpr (T::kRowMajor) {
           if (args.tma_store) {
             // 32 rows x 32 columns as a 64-byte-swizzled box for a TMA store
             const uint32_t slab = slab0 + (stores & (kMxSlabs - 1)) * kMxSlabBytes;
@@ -521,7 +523,7 @@ __global__ void __launch_bounds__(224) mx_gemm_kernel(const __grid_constant__ CU
         store_rest(0, BN);
       }
     }
-    if (lane == 0) ptx::tma_store_wait<0>();
+    if (T::kRowMajor && lane == 0) ptx::tma_store_wait<0>();
     __syncwarp();
   }
 
