@@ -252,6 +252,9 @@ int b200_mx_dequantize(int format, int f16, int rows, int cols, const void* data
   args.pitch = mx_pitch(cols);
   args.col_tiles = mx_col_tiles(cols);
   args.tensor_scale = tensor_scale;
+  uint32_t bits;
+  std::memcpy(&bits, &tensor_scale, sizeof bits);
+  args.inexact = (bits & 0x007FFFFFu) != 0 ? 1 : 0;
   args.x = static_cast<uint16_t*>(X);
   args.ldx = ldx;
   const long long tiles_x = (cols + kQuantTile - 1) / kQuantTile, tiles_y = mx_row_tiles(rows);

@@ -15,8 +15,8 @@
 // takes 128 x 128 elements: 256 bytes of every row (whole lines), eight 16-byte loads in flight per
 // thread, and complete 512-byte scale groups in either direction, so scales leave as whole lines and
 // the padding of the scale layout is written by the CTAs at the edges instead of a memset. The
-// transposed form turns the tile in shared memory (34 KB, so six CTAs per SM); both forms at once
-// read the matrix once.
+// transposed form turns the tile in shared memory (34 KB; with 48 to 64 registers per thread four or five CTAs
+// per SM); both forms at once read the matrix once.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -351,20 +351,31 @@ struct DequantArgs {
   const uint8_t* scales;
   long long rows, cols, pitch, col_tiles;
   float tensor_scale;
+  int inexact;              // 1: the tensor scale is no power of two
   uint16_t* x;
   long long ldx;
   int tiles_x;
 };
 
+// v * t, where fp32 has to round it, rounded to odd: the last bit says that something was cut off, so the rounding to 16 bits
+// that follows is the only one. (Below fp32's normal numbers what was cut off may be lost.)
+__device__ __forceinline__ float product_to_odd(float v, float t) {
+  const float p = __fmul_rn(v, t);
+  const float rest = fmaf(v, t, -p);
+  if (rest == 0.0f) return p;
+  const uint32_t bits = __float_as_uint(p) - ((rest < 0.0f) != (p < 0.0f) ? 1u : 0u);  // towards zero
+  return __uint_as_float(bits | 1u);
+}
+
 template <int FMT, int F16>
-__device__ __forceinline__ void dequantise8(uint32_t (&w)[4], uint32_t codes, float scale, float tensor_scale) {
+__device__ __forceinline__ void dequantise8(uint32_t (&w)[4], uint32_t codes, float scale, float tensor_scale, int inexact) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     float lo = e2m1_value(codes >> (8 * j)) * scale;
     float hi = e2m1_value(codes >> (8 * j + 4)) * scale;
     if constexpr (FMT == kNvfp4) {
-      lo *= tensor_scale;
-      hi *= tensor_scale;
+      lo = inexact ? product_to_odd(lo, tensor_scale) : lo * tensor_scale;
+      hi = inexact ? product_to_odd(hi, tensor_scale) : hi * tensor_scale;
     }
     if constexpr (F16) {
       asm("cvt.rn.f16x2.f32 %0, %2, %1;" : "=r"(w[j]) : "f"(lo), "f"(hi));
@@ -374,8 +385,8 @@ __device__ __forceinline__ void dequantise8(uint32_t (&w)[4], uint32_t codes, fl
   }
 }
 
-// Codes and scales -> 16-bit values: code * scale * tensor scale in fp32, rounded once (exact in bf16
-// unless it leaves bf16's range: 2 bits of code times at most 4 of scale). Same 128 x 128 tiles.
+// Codes and scales -> 16-bit values: code * scale * tensor scale in fp32, rounded once (under a tensor scale that is a power
+// of two exact in bf16 unless it leaves bf16's range: 2 bits of code times at most 4 of scale). Same 128 x 128 tiles.
 template <int FMT, int F16, int VEC>
 __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_constant__ DequantArgs args) {
   const int t = static_cast<int>(threadIdx.x);
@@ -412,7 +423,7 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_
     if (row >= args.rows || col >= args.cols) continue;
     const float scale = mx_scale_value<FMT>((scales[p & 1][p / 2] >> (8 * static_cast<int>(block % 4))) & 0xFFu);
     uint32_t w[4];
-    dequantise8<FMT, F16>(w, codes[p], scale, args.tensor_scale);
+    dequantise8<FMT, F16>(w, codes[p], scale, args.tensor_scale, args.inexact);
     if constexpr (VEC) {
       uint16_t* dst = args.x + row * args.ldx + col;
       if (col + 8 <= args.cols) {
@@ -438,7 +449,7 @@ __global__ void __launch_bounds__(kQuantThreads) dequantize_kernel(const __grid_
         const uint32_t word = *reinterpret_cast<const uint32_t*>(args.data + row * args.pitch + next / 2);
         const uint32_t byte = args.scales[mx_scale_offset(FMT, row, next / mx_block(FMT), args.col_tiles)];
         uint32_t w[4];
-        dequantise8<FMT, F16>(w, word, mx_scale_value<FMT>(byte), args.tensor_scale);
+        dequantise8<FMT, F16>(w, word, mx_scale_value<FMT>(byte), args.tensor_scale, args.inexact);
         *reinterpret_cast<uint4*>(tile + t * kQuantPitch + kQuantTile * 2) = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }

@@ -153,3 +153,24 @@ def test_sizes_beyond_32_bits_are_refused():
         with pytest.raises(g.GemmError, match="hidden and inner"):
             g.moe_layer(meta(1, H), meta(2, H), meta(2, 2 * I, H), meta(2, H, I), 1)
         assert g.moe_workspace_bytes(1, 2, 1, H, I) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [64, 67])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_values_read_back_are_rounded_once(dtype, cols):
+    """Tensor scales that put code * scale next to the middle between two 16-bit numbers, nearer than fp32 can tell."""
+    half = torch.finfo(dtype).eps / 2
+    code = torch.full((1, (cols + 1) // 2), 5 | 13 << 4, dtype=torch.uint8)           # 3 and -3
+    block = torch.full((1, -(-cols // 16)), 0x38, dtype=torch.uint8)                   # 1
+    sides = set()
+    for k in range(40):
+        middle = 1 + half * (2 * k + 1)
+        ts = torch.tensor(middle / 3, dtype=torch.float64).float().double().item()
+        q = g.MxTensor.from_parts(code.cuda(), block.cuda(), cols, "nvfp4", ts)
+        value = 3 * ts                                                               # exact in 64 bits
+        sides.add((value > middle) - (value < middle))
+        want = torch.tensor(1 + 2 * half * (k + (value > middle) + (value == middle) * (k % 2)), dtype=torch.float64)
+        got = g.dequantize_mx(q, dtype).double().cpu()[0]
+        assert (got[0::2] == want).all() and (got[1::2] == -want).all(), (k, got[:2], want)
+    assert {-1, 1} <= sides
