@@ -35,7 +35,7 @@ def moe_layer(x, router, w_gate_up, w_down, top_k: int, bias=None, renormalize: 
 
     With ``return_routing`` the result is ``(out, ids, weights)``: the chosen experts [T, top_k] (int32, largest
     logit first, -1 where fewer experts than top_k are left) and their weights (fp32). A token without any
-    expert gets zeros. Expert weights have to be finite. With float16 a hidden value beyond 65504 is infinite.
+    expert gets zeros. No history for gradients is recorded. Expert weights have to be finite. With float16 a hidden value beyond 65504 is infinite.
     include/b200_gemm.h has the rounding and the limits.
     """
     f16 = _half_type(x.dtype, "x")

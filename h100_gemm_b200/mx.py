@@ -13,6 +13,9 @@ blocks have to run along the contraction::
     dr, dc = quantize_mx_both(dy)           # [M, N], [N, M]
     dx = gemm_mx(dr, wc)                    # [M, K], over N
     dw = gemm_mx(dc, xc)                    # [N, K], over M
+
+No call here records a history: results of tensors that require gradients do not, and a backward pass is made of the
+calls above (in a torch.autograd.Function of the caller's, for instance).
 """
 from __future__ import annotations
 
