@@ -22,6 +22,16 @@ bool sizes_ok(int T, int E, int k, int H, int I) {
 // What b200_mx_dequantize takes.
 bool weights_scale_ok(int format, float t) { return t > 0.0f && t <= 3.4e38f && (format == B200_NVFP4 || t == 1.0f); }
 
+// lift (a power of two) times the tensor scale in one number, unless that leaves fp32's range: then 2^32 of it apart.
+void split_factor(float (&factor)[2], float lift, float tensor_scale) {
+  factor[0] = lift * tensor_scale;
+  factor[1] = 1.0f;
+  if (factor[0] > 3.4e38f) {
+    factor[0] = tensor_scale * (lift * 0x1p-32f);
+    factor[1] = 0x1p32f;
+  }
+}
+
 template <int W, int F16>
 int launch_all(const DeviceInfo& dev, const MoeArgs& args, cudaStream_t stream) {
   static std::atomic<bool> up_allowed[64], down_allowed[64];
@@ -116,8 +126,9 @@ int b200_moe_layer(int f16, int T, int E, int top_k, int H, int I, const void* X
   args.w2.scales = static_cast<const uint8_t*>(W2_scales);
   args.w2.pitch = four_bit ? mx_pitch(I) : 2ll * I;
   args.w2.col_tiles = mx_col_tiles(I);
-  args.scale1 = four_bit ? W1_tensor_scale : 1.0f;
-  args.scale2 = four_bit ? W2_tensor_scale : 1.0f;
+  const float lift = weight_format == B200_NVFP4 ? MoeUnit<kMoeNvfp4, 0>::kLift : 1.0f;
+  split_factor(args.scale1, lift, four_bit ? W1_tensor_scale : 1.0f);
+  split_factor(args.scale2, lift, four_bit ? W2_tensor_scale : 1.0f);
   args.h = reinterpret_cast<uint16_t*>(ws);
   args.ids = ids != nullptr ? ids : reinterpret_cast<int*>(ws + h_bytes(T, top_k, I));
   args.weights = weights != nullptr ? weights : reinterpret_cast<float*>(ws + h_bytes(T, top_k, I) + pair_bytes(T, top_k));

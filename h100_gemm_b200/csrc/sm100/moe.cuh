@@ -55,7 +55,7 @@ struct MoeArgs {
   const float* bias;        // [E] or NULL
   MoeMatrix w1;             // [E, 2 I, H]: gate rows, then up rows
   MoeMatrix w2;             // [E, H, I]
-  float scale1, scale2;     // tensor scales of w1 and w2 (1 for 16-bit weights)
+  float scale1[2], scale2[2];  // two factors each of what sums of products with w1 / w2 are multiplied with
   int* ids;                 // [T, k], -1 = none
   float* weights;           // [T, k]
   uint16_t* h;              // [T, k, 2, I]: HiddenParts
@@ -850,7 +850,6 @@ struct GateUp {
   static constexpr int kCols = 8 * MT;
   using Weights = typename MoeUnit<W, F16>::GateUp;
   static constexpr int kStep = Weights::kStep;
-  static constexpr float kLift = MoeUnit<W, F16>::kLift;  // (a power of two, and applied by itself: with the tensor scale it may leave fp32's range)
   const MoeArgs& args;
   const RouteTables& r;
   uint32_t lane;
@@ -926,7 +925,7 @@ struct GateUp {
         gate += at[p * stride * 4];
         up += at[p * stride * 4 + 2];
       }
-      const float h = r.weights[first_pair + c] * (silu(gate * kLift * args.scale1) * (up * kLift * args.scale1));
+      const float h = r.weights[first_pair + c] * (silu(gate * args.scale1[0] * args.scale1[1]) * (up * args.scale1[0] * args.scale1[1]));
       uint16_t* to = args.h + static_cast<long long>(r.pairs[first_pair + c]) * 2 * args.I + MoeUnit<W, F16>::Down::hidden_place(row);
       HiddenParts<F16>::store(h, to, to + args.I);
     }
@@ -1090,7 +1089,7 @@ __global__ void __launch_bounds__(kMoeThreads, 2) moe_down_kernel(const __grid_c
     float v = 0.0f;
 #pragma unroll 4
     for (int p = 0; p < split; ++p) v += ptx::ld_cluster_f32(split > 1 ? ptx::map_to_cta(addr + at, p) : addr + at);
-    if (d.r0 + row < args.H) args.out[static_cast<long long>(t) * args.H + d.r0 + row] = round16<F16>(v * MoeUnit<W, F16>::kLift * args.scale2);
+    if (d.r0 + row < args.H) args.out[static_cast<long long>(t) * args.H + d.r0 + row] = round16<F16>(v * args.scale2[0] * args.scale2[1]);
   }
   if (split > 1) {
     ptx::cluster_arrive();  // no CTA leaves while another reads its sums

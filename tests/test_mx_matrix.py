@@ -122,7 +122,7 @@ def test_products_under_far_tensor_scales():
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("e1,e2", [(100, 112), (-100, -100)])
+@pytest.mark.parametrize("e1,e2", [(100, 112), (-100, -100), (-124, -100)])
 def test_experts_under_far_tensor_scales(e1, e2):
     """NVFP4 experts whose tensor scales are far from 1, undone by the tokens (gate and up) or seen in the result."""
     T, E, k, H, I = 3, 4, 2, 64, 48
