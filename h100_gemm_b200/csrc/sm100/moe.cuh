@@ -872,6 +872,7 @@ struct GateUp {
       b[j] = args.x + static_cast<long long>(r.tokens[first_pair + c]) * args.H;
     }
     float acc[NT][MT][4] = {};
+    __syncwarp();  // (the MMA wants all lanes together; the sums before it were written under a condition)
     w.mma_tokens(acc, b, k0, args.H, lane);
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -1002,6 +1003,7 @@ struct Down {
     const int token = min(c0 + column / kWidth, tokens - 1);
     const Hidden columns(args.h + static_cast<long long>(r.pairs[first_pair + token]) * 2 * args.I, args.I, column);
     float acc[Hidden::kSums][MT][4] = {};
+    __syncwarp();  // (as for the gate/up product)
     w.mma_hidden(acc, columns, k0, args.I, lane);
     // A lane holds columns 2 (lane % 4) and the next one, of rows lane / 4 + 8 m.
     const auto add = [&](int c, auto part) {

@@ -22,6 +22,15 @@ def test_lanes_meet_before_every_aligned_cluster_barrier():
     assert issued == 2
 
 
+def test_lanes_meet_before_the_expert_layers_mmas():
+    """mma.sync.aligned is undefined for a warp in parts, and sums are written lane by lane under conditions before it."""
+    text = (SM100 / "moe.cuh").read_text()
+    calls = list(re.finditer(r"\n    w\.mma_(tokens|hidden)\(", text))
+    assert len(calls) == 2
+    for m in calls:
+        assert "__syncwarp();" in text[:m.start()].rsplit("\n", 1)[1], m.group(0)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T", [1, 2, 3, 5, 7])
